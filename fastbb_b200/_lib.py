@@ -43,6 +43,11 @@ class BlockDesc(ctypes.Structure):
                 + [(n, _f32) for n in ("eps1", "eps2", "scale")])
 
 
+class RotaryTensor(ctypes.Structure):
+    """fbb_rotary_tensor of include/fastbb_b200.h: one tensor to turn, [B, N, heads, D], and where to."""
+    _fields_ = [("x", _vp), ("y", _vp), ("heads", _i32)] + [(n, _i64) for n in ("x_sb", "x_sn", "x_sh", "y_sb", "y_sn", "y_sh")]
+
+
 MLP_GELU, MLP_SWIGLU = 0, 1
 _bdp = ctypes.POINTER(BlockDesc)
 
@@ -67,6 +72,7 @@ PROTOTYPES = {
     "fbb_flash64_launches": (_i32, [_i32, _i32, _i32, _i32]),
     "fbb_flash64_f16_ws": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _i32] + [_i64] * 12 + [_f32, _i32, _vp, _i64, _vp]),
     "fbb_flash64_f16_static": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _i32] + [_i64] * 12 + [_f32, _i32, _vp]),
+    "fbb_rotary": (_i32, [ctypes.POINTER(RotaryTensor)] + [_i32] * 7 + [_vp, _i32, _i32, _i64, _i64, _i64, _vp, _vp, _i32, _i32, _vp]),
     "fbb_stack_scratch_bytes": (_i64, [_bdp, _i32, _i64]),
     "fbb_stack_launches": (_i32, [_bdp, _i32, _i64]),
     "fbb_stack_forward_f16": (_i32, [_bdp, _i32, _vp, _i32, _i32, _vp, _i64, _vp, _i64, _vp]),
@@ -133,6 +139,47 @@ def stream_ptr(device=None):
 
 def ptr(t):
     return t.data_ptr() if t is not None else None
+
+
+def _nested(t):
+    """(size, stride) of t's dimensions of more than one element, innermost first, and whether no two elements share an address
+    (every stride steps over what the dimensions inside it span)."""
+    dims = sorted(((n, s) for n, s in zip(t.shape, t.stride()) if n > 1), key=lambda d: d[1])
+    span, ok = 1, True
+    for n, s in dims:
+        ok = ok and s >= span
+        span += (n - 1) * s
+    return dims, ok
+
+
+def writable(t):
+    """Whether every element of t has an address of its own (an expanded or self-overlapping view cannot be written by many threads)."""
+    return t.numel() == 0 or _nested(t)[1]
+
+
+def same_view(a, b):
+    return a.data_ptr() == b.data_ptr() and a.shape == b.shape and a.dtype == b.dtype and all(
+        n == 1 or s == r for n, s, r in zip(a.shape, a.stride(), b.stride()))
+
+
+def disjoint(a, b):
+    """Whether a and b (of one dtype) surely share no element: other storages, byte ranges apart, or views of one buffer that lie beside
+    each other within equal outer strides, like the queries and keys of a packed projection."""
+    if a.numel() == 0 or b.numel() == 0 or a.untyped_storage().data_ptr() != b.untyped_storage().data_ptr():
+        return True
+    if a.data_ptr() > b.data_ptr():
+        a, b = b, a
+    gap = (b.data_ptr() - a.data_ptr()) // a.element_size()
+    da, db = _nested(a)[0], _nested(b)[0]
+    for k in range(len(da) + 1):  # the k innermost dimensions of a against what the outer ones leave for b
+        outer = da[k:]
+        m = len(db) - len(outer)
+        if m < 0 or db[m:] != outer:
+            continue
+        span_a, span_b = 1 + sum((n - 1) * s for n, s in da[:k]), 1 + sum((n - 1) * s for n, s in db[:m])
+        if gap >= span_a and (not outer or gap + span_b <= outer[0][1]):
+            return True
+    return 1 + sum((n - 1) * s for n, s in da) <= gap
 
 
 def device_status():

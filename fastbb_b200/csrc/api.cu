@@ -278,6 +278,33 @@ int fbb_linear_layernorm_f16(const void* A, const void* W, void* C, const void* 
                                    counter, (cudaStream_t)stream);
 }
 
+int fbb_rotary(const fbb_rotary_tensor* tensors, int n_tensors, int B, int N, int D, int pairs, int pairing, int n_prefix, const void* positions,
+               int pos_dtype, int n_axes, int64_t p_sb, int64_t p_sn, int64_t p_sa, const float* freqs, const int* axes, int inverse, int dtype,
+               void* stream) {
+    if (tensors == nullptr || freqs == nullptr || axes == nullptr) return fail(FBB_ERR_NULL, "rotary: tensors, freqs or axes is null");
+    if (n_tensors < 1 || n_tensors > 2) return fail(FBB_ERR_SHAPE, "rotary: one or two tensors, got %d", n_tensors);
+    if (dtype < FBB_DTYPE_F16 || dtype > FBB_DTYPE_F32 || pos_dtype < FBB_POS_I32 || pos_dtype > FBB_POS_F32)
+        return fail(FBB_ERR_ENUM, "rotary: unknown dtype code (values %d, positions %d)", dtype, pos_dtype);
+    if (pairing != FBB_ROTARY_HALF && pairing != FBB_ROTARY_PAIRS) return fail(FBB_ERR_ENUM, "rotary: unknown pairing %d", pairing);
+    if (B < 0 || N < 0 || D <= 0 || D > 1024 || pairs < 1 || 2 * (int64_t)pairs > D || n_axes < 1 || n_prefix < 0 || (int64_t)B * N > 0x7FFFFFFFll)
+        return fail(FBB_ERR_SHAPE, "rotary: bad sizes (B=%d N=%d D=%d pairs=%d axes=%d prefix=%d)", B, N, D, pairs, n_axes, n_prefix);
+    const uintptr_t unit = dtype == FBB_DTYPE_F32 ? 3u : 1u;
+    for (int i = 0; i < n_tensors; ++i) {
+        if (tensors[i].heads < 1 || tensors[i].heads > 65535) return fail(FBB_ERR_SHAPE, "rotary: bad number of heads %d", tensors[i].heads);
+        if (B == 0 || N == 0) continue;
+        if (tensors[i].x == nullptr || tensors[i].y == nullptr) return fail(FBB_ERR_NULL, "rotary: x or y of tensor %d is null", i);
+        if ((reinterpret_cast<uintptr_t>(tensors[i].x) & unit) || (reinterpret_cast<uintptr_t>(tensors[i].y) & unit))
+            return fail(FBB_ERR_ALIGN, "rotary: x and y must be aligned to their elements");
+    }
+    if (B == 0 || N == 0) return FBB_OK;
+    if (N > n_prefix) {
+        if (positions == nullptr) return fail(FBB_ERR_NULL, "rotary: positions is null");
+        if (reinterpret_cast<uintptr_t>(positions) & (pos_dtype == FBB_POS_I64 ? 7u : 3u)) return fail(FBB_ERR_ALIGN, "rotary: positions must be aligned to their elements");
+    }
+    return launch_rotary(tensors, n_tensors, B, N, D, pairs, pairing, n_prefix, positions, pos_dtype, n_axes, p_sb, p_sn, p_sa, freqs, axes, inverse,
+                         dtype, (cudaStream_t)stream);
+}
+
 #endif  // FBB_FLASH_ONLY
 
 int64_t fbb_flash64_workspace_bytes(int B, int N, int H) { return flash64_workspace_bytes_for(B, N, H); }

@@ -3,5 +3,6 @@
 #include "layernorm.cu"
 #include "gemm.cu"
 #include "flash64.cu"
+#include "rotary.cu"
 #include "block.cu"
 #include "api.cu"

@@ -102,6 +102,9 @@ int flash64_static_workspace(void** ptr, int64_t* bytes, cudaStream_t stream);
 int64_t flash64_workspace_bytes_for(int B, int N, int H);
 int flash64_launches(int B, int N, int H, bool has_workspace);
 
+int launch_rotary(const fbb_rotary_tensor* t, int n_tensors, int B, int N, int D, int pairs, int pairing, int n_prefix, const void* pos, int pos_dtype,
+                  int n_axes, int64_t p_sb, int64_t p_sn, int64_t p_sa, const float* freqs, const int* axes, int inverse, int dtype, cudaStream_t stream);
+
 // One FFI crossing per block / stack (block.cu): scratch needed for `tokens` tokens, and the launches themselves.
 int64_t stack_scratch_bytes(const fbb_block_desc* d, int n_blocks, int64_t tokens);
 int stack_launches(const fbb_block_desc* d, int n_blocks, int64_t tokens);  // kernels stack_forward enqueues for this run

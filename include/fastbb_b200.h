@@ -192,6 +192,30 @@ int fbb_flash64_f16_static(const void* q, const void* k, const void* v, void* o,
                            int64_t q_sh, int64_t k_sb, int64_t k_sn, int64_t k_sh, int64_t v_sb, int64_t v_sn, int64_t v_sh,
                            int64_t o_sb, int64_t o_sn, int64_t o_sh, float scale, int variant, void* stream);
 
+/* ---- rotary positions ---------------------------------------------------------------------------------------------------
+ * Queries and keys turned by the positions of their tokens on one or several axes, one launch for both. No counterpart in the
+ * reference (its models have learned position tables); it stands between fbb_linear_f16 (qkv) and fbb_flash64_f16.
+ * Pair i < pairs of every head's D columns, in a row whose position on axis axes[i] is p, is turned by t = p * freqs[i]:
+ *   (x, y) -> (x cos t - y sin t, y cos t + x sin t), or by -t with inverse != 0 (the transposed rotation: the gradient's).
+ * FBB_ROTARY_HALF: a pair is columns (i, i + pairs); FBB_ROTARY_PAIRS: columns (2i, 2i + 1). Columns from 2 * pairs on and the
+ * first n_prefix rows of every sequence pass unchanged. Angles are products in 64 bits, reduced before sine and cosine in 32;
+ * the rotation is fp32, rounded once.
+ * tensors: one or two of {x, y, heads, strides of [B, N, heads, D] in elements, D contiguous}; y may be x itself, otherwise it
+ * shares no memory with any x. positions: [B, N - n_prefix, n_axes] of pos_dtype with strides p_sb, p_sn, p_sa (p_sb 0: the same
+ * for every sequence). freqs: [pairs] fp32, axes: [pairs] int32, both in device memory; an axis out of [0, n_axes) is clamped.
+ * Any size, stride and alignment of whole elements; multiples of 16 bytes take the vector form. D <= 1024, B * N < 2^31. */
+enum fbb_rotary_pairing { FBB_ROTARY_HALF = 0, FBB_ROTARY_PAIRS = 1 };
+enum fbb_pos_dtype { FBB_POS_I32 = 0, FBB_POS_I64 = 1, FBB_POS_F32 = 2 };
+typedef struct fbb_rotary_tensor {
+    const void* x;
+    void* y;
+    int heads;
+    int64_t x_sb, x_sn, x_sh, y_sb, y_sn, y_sh;
+} fbb_rotary_tensor;
+int fbb_rotary(const fbb_rotary_tensor* tensors, int n_tensors, int B, int N, int D, int pairs, int pairing, int n_prefix, const void* positions,
+               int pos_dtype, int n_axes, int64_t p_sb, int64_t p_sn, int64_t p_sa, const float* freqs, const int* axes, int inverse, int dtype,
+               void* stream);
+
 /* ---- one FFI crossing per transformer block or per run of blocks -------------------------------------------------------
  * Replaces FastViT.block / block_chunked and the loop over blocks in FastViT.run (fastbb/vit.py:108-172, 175-187), which
  * cross from Python into torch / ctypes ten to eleven times per block. The same seven kernels are enqueued in the same

@@ -1,0 +1,248 @@
+"""rotary(): against the rotation in 64 bits over sizes, layouts, types and pairings; in place; refusals.
+
+Tolerance. The angle's fraction of a turn is rounded to fp32 (half a step of 2^-25 at most: 2^-26 turns, 2^-23.3 radians), sine and
+cosine are off by up to 2 steps (2^-23), the two products and their sum by one rounding each (2^-24 of |x| + |y| twice): together
+less than (|x| + |y|) 2^-21. The result is rounded to its type once: half a step of it, eps / 2 relative, or half of the smallest
+subnormal."""
+import math
+
+import pytest
+import torch
+
+from fastbb_b200 import _lib
+from fastbb_b200.rotary import RotaryPlan, axial_plan, grid_positions, rotary, rotary_plan
+
+
+def reference(x, positions, plan, n_prefix, inverse):
+    x = x.double().cpu()
+    pos = positions.double().cpu()
+    pos = pos if pos.dim() == 3 else pos.expand(x.shape[0], *pos.shape)
+    angle = pos[..., plan.axes.cpu().long()] * plan.freqs.double().cpu()
+    if inverse:
+        angle = -angle
+    c, s = angle.cos()[:, :, None], angle.sin()[:, :, None]
+    p = plan.freqs.numel()
+    out = x.clone()
+    body = x[:, n_prefix:]
+    a, b = (slice(0, p), slice(p, 2 * p)) if plan.pairing == "half" else (slice(0, 2 * p, 2), slice(1, 2 * p, 2))
+    out[:, n_prefix:, :, a] = body[..., a] * c - body[..., b] * s
+    out[:, n_prefix:, :, b] = body[..., b] * c + body[..., a] * s
+    room = torch.zeros_like(x)
+    room[:, n_prefix:, :, a] = room[:, n_prefix:, :, b] = body[..., a].abs() + body[..., b].abs()
+    return out, room
+
+
+def check(got, x, positions, plan, n_prefix=0, inverse=False):
+    want, room = reference(x, positions, plan, n_prefix, inverse)
+    info = torch.finfo(got.dtype)
+    limit = room * 2.0 ** -21 + want.abs() * info.eps / 2 * (room > 0) + info.smallest_normal * info.eps / 2 * (room > 0)
+    over = (got.double().cpu() - want).abs() - limit
+    assert bool((over <= 0).all()), f"{int((over > 0).sum())} of {over.numel()} off, worst by {float(over.max()):.3g}"
+
+
+def tensor(shape, dtype, layout, g):
+    """A [B, N, H, D] view of the wanted layout."""
+    B, N, H, D = shape
+    if layout == "plain":
+        return torch.randn(shape, generator=g).to(dtype).cuda()
+    if layout == "heads":        # [B, H, N, D] in memory
+        return torch.randn(B, H, N, D, generator=g).to(dtype).cuda().transpose(1, 2)
+    if layout == "odd":          # rows of an odd number of elements, from an odd element on
+        return torch.randn(B, N, H, D + 3, generator=g).to(dtype).cuda()[..., 1:D + 1]
+    if layout == "wide":         # every other row and head of a larger buffer
+        return torch.randn(B, 2 * N, 2 * H, D, generator=g).to(dtype).cuda()[:, ::2, 1::2]
+    raise AssertionError(layout)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("pairing", ["half", "pairs"])
+@pytest.mark.parametrize("B,N,H,Hk,D,pairs,prefix,layout", [
+    (1, 1, 1, 1, 64, 32, 0, "plain"), (1, 1, 3, 1, 64, 32, 1, "plain"), (2, 5, 6, 2, 64, 32, 1, "heads"), (3, 37, 12, 4, 80, 40, 0, "plain"),
+    (1, 257, 6, 6, 64, 32, 1, "plain"), (2, 19, 4, 2, 128, 32, 5, "wide"), (1, 33, 5, 5, 64, 24, 0, "plain"), (2, 9, 3, 3, 20, 7, 2, "plain"),
+    (1, 16, 2, 1, 64, 32, 0, "odd"), (1, 7, 2, 2, 2, 1, 0, "plain"), (1, 3, 2, 1, 1024, 512, 0, "plain"), (2, 40, 24, 24, 64, 32, 4, "plain"),
+    (1, 700, 16, 16, 64, 32, 1, "plain")])
+def test_matches_the_rotation_in_64_bits(B, N, H, Hk, D, pairs, prefix, layout, pairing, dtype):
+    g = torch.Generator().manual_seed(N * 7 + D)
+    q, k = tensor((B, N, H, D), dtype, layout, g), tensor((B, N, Hk, D), dtype, layout, g)
+    axes = 1 + (N + D) % 3
+    plan = rotary_plan([100.0 ** (-i / pairs) for i in range(pairs)], [i % axes for i in range(pairs - 1)] + [axes - 1] if pairs > 1 else [0], pairing=pairing)
+    where = torch.randn(B, N - prefix, plan.n_axes, generator=g).mul_(30).cuda()
+    if N % 2:
+        where = where[0]
+    for inverse in (False, True):
+        q2, k2 = rotary(q, k, where, plan, n_prefix=prefix, inverse=inverse)
+        check(q2, q, where, plan, prefix, inverse)
+        check(k2, k, where, plan, prefix, inverse)
+    only, none = rotary(q, None, where, plan, n_prefix=prefix, inverse=True)
+    assert none is None and torch.equal(only, q2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64, torch.float32])
+def test_far_positions_of_every_type(dtype):
+    g = torch.Generator().manual_seed(3)
+    q = torch.randn(1, 64, 2, 64, generator=g).cuda()
+    plan = axial_plan(64, axes=2, theta=10000.0)
+    far = 2 ** 31 - 129 if dtype != torch.float32 else 2 ** 24 - 64
+    where = torch.stack((torch.arange(64), far + torch.arange(64)), -1)
+    where = where.to(dtype).cuda()
+    check(rotary(q, None, where, plan)[0], q, where, plan)
+    check(rotary(q, None, -where, plan)[0], q, -where, plan)
+    strided = torch.stack((where, torch.zeros_like(where)), 1).transpose(0, 1)[0]          # positions of strides of their own
+    assert torch.equal(rotary(q, None, strided, plan)[0], rotary(q, None, where, plan)[0])
+    columns = where.t().contiguous().t()
+    assert torch.equal(rotary(q, None, columns, plan)[0], rotary(q, None, where, plan)[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pairing", ["half", "pairs"])
+def test_in_place_on_the_packed_projection_leaves_the_rest(pairing):
+    g = torch.Generator().manual_seed(5)
+    qkv = torch.randn(2, 38, 3, 6, 64, generator=g).half().cuda()
+    before = qkv.clone()
+    plan, where = axial_plan(64, unit=2 * math.pi, pairing=pairing), grid_positions(4, 8)
+    q, k, v = qkv.unbind(2)
+    want = rotary(q, k, where, plan, n_prefix=6)
+    got = rotary(q, k, where, plan, n_prefix=6, out=(q, k))
+    assert got[0] is q and got[1] is k
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1])
+    assert torch.equal(v, before[:, :, 2]) and torch.equal(qkv[:, :6], before[:, :6])
+    back = rotary(q, k, where, plan, n_prefix=6, inverse=True)
+    assert float((back[0] - before[:, :, 0]).abs().max()) < 2 ** -8
+
+
+@pytest.mark.gpu
+def test_passing_rows_and_columns_keep_their_bits():
+    g = torch.Generator().manual_seed(6)
+    q = torch.randn(1, 12, 2, 64, generator=g).half().cuda()
+    q[:, :3] = torch.tensor([float("inf"), float("nan"), -0.0, 65504.0]).half().cuda().repeat(16)
+    q[..., 48:] = float("nan")
+    plan = rotary_plan([0.5] * 24, [0] * 24)
+    out = rotary(q, None, torch.arange(9, device="cuda").view(9, 1), plan, n_prefix=3)[0]
+    assert torch.equal(out[:, :3].view(torch.int16), q[:, :3].view(torch.int16))
+    assert torch.equal(out[..., 48:].view(torch.int16), q[..., 48:].view(torch.int16))
+    check(out[:, 3:, :, :48], q[:, 3:, :, :48], torch.arange(9).view(9, 1), plan)
+
+
+@pytest.mark.gpu
+def test_gradients_against_the_formula_and_differences():
+    """With loss = sum(w * rotary(x)) the gradient is the inverse rotation of w; the loss is linear in x, so a difference is exact up
+    to the roundings: fp32 sums of 12 * 2 * 64 products of size about 1, 2^-24 each."""
+    g = torch.Generator().manual_seed(7)
+    x, w = torch.randn(1, 12, 2, 64, generator=g).cuda(), torch.randn(1, 12, 2, 64, generator=g).cuda()
+    plan, where = axial_plan(64, unit=3.0), grid_positions(3, 4)
+    grad = rotary(w, None, where, plan, inverse=True)[0]
+    check(grad, w, where, plan, inverse=True)
+    step = torch.randn(1, 12, 2, 64, generator=g).cuda()
+    high, low = rotary(x + step, None, where, plan)[0], rotary(x - step, None, where, plan)[0]
+    difference = float(((high.double() - low.double()) * w.double()).sum()) / 2
+    along = float((grad.double() * step.double()).sum())
+    assert abs(difference - along) < 12 * 2 * 64 * 4 * 2.0 ** -21
+
+
+@pytest.mark.gpu
+def test_other_stream_and_captured_graph():
+    g = torch.Generator().manual_seed(8)
+    q = torch.randn(1, 65, 6, 64, generator=g).half().cuda()
+    plan, where = axial_plan(64), grid_positions(8, 8)
+    want = rotary(q, q, where, plan, n_prefix=1)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = rotary(q, None, where, plan, n_prefix=1)[0]
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(other, want[0])
+    held = torch.zeros_like(q)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = rotary(held, None, where, plan, n_prefix=1)[0]
+    for scale in (1.0, -2.0):
+        held.copy_(q * scale)
+        graph.replay()
+        assert torch.equal(captured, rotary(q * scale, None, where, plan, n_prefix=1)[0])
+
+
+@pytest.mark.gpu
+def test_empty_calls_and_no_rows_with_positions():
+    plan = axial_plan(64)
+    for shape in ((0, 5, 2, 64), (3, 0, 2, 64)):
+        q = torch.zeros(shape, dtype=torch.float16, device="cuda")
+        assert rotary(q, None, torch.zeros(shape[1], 2, device="cuda"), plan)[0].shape == shape
+    q = torch.randn(2, 3, 2, 64, device="cuda")
+    assert torch.equal(rotary(q, None, torch.zeros(0, 2, device="cuda"), plan, n_prefix=3)[0], q)
+
+
+@pytest.mark.gpu
+def test_refusals_on_the_gpu():
+    plan, where = axial_plan(64), grid_positions(2, 4)
+    qkv = torch.zeros(1, 8, 3, 2, 64, dtype=torch.float16, device="cuda")
+    q, k, v = qkv.unbind(2)
+    wide = torch.zeros(1, 8, 2, 64, dtype=torch.float16, device="cuda").expand(4, 8, 2, 64)
+    for call in (
+            lambda: rotary(q, k, where[:5], plan), lambda: rotary(q, k, where, plan, n_prefix=1), lambda: rotary(q, k, where, plan, n_prefix=9),
+            lambda: rotary(q, k.float(), where, plan), lambda: rotary(q, k[:, :4], where, plan), lambda: rotary(q.double(), None, where, plan),
+            lambda: rotary(q, k, where.half(), plan), lambda: rotary(q, k, where.cpu(), plan), lambda: rotary(q[..., ::2], None, where, plan),
+            lambda: rotary(q, k, where, plan, out=(k, q)), lambda: rotary(q, k, where, plan, out=(q, q)), lambda: rotary(q, k, where, plan, out=(v, v)),
+            lambda: rotary(q, None, where, plan, out=(qkv[:, :, 0:2].flatten(2, 3)[:, :, 1:3],)), lambda: rotary(q, k, where, plan, out=(q,)),
+            lambda: rotary(wide, None, where, plan, out=(wide,)), lambda: rotary(q, k, where, axial_plan(128)),
+            lambda: rotary(q, k, where, axial_plan(64, axes=3)), lambda: rotary(q, k, where, axial_plan(64, device="cpu")),
+            lambda: rotary(q, k, where, RotaryPlan(plan.freqs, plan.axes, 2, "thirds"))):
+        with pytest.raises(ValueError):
+            call()
+    assert torch.equal(rotary(q, k, where, plan, out=(v, torch.empty_like(k)))[0], q)  # another part of the buffer is fine
+
+
+# ------------------------------------------------------------------------------------------------------------------ CPU
+def test_plans():
+    plan = axial_plan(64, axes=3, theta=50.0, unit=2.0, shares=[8, 12, 12], device="cpu")
+    assert plan.n_axes == 3 and plan.axes.tolist() == [0] * 8 + [1] * 12 + [2] * 12
+    assert plan.freqs[0] == plan.freqs[8] == plan.freqs[20] == 2.0 and math.isclose(float(plan.freqs[9]), 2.0 * 50.0 ** (-1 / 12), rel_tol=1e-6)
+    ladder = axial_plan(64, axes=3, theta=50.0, shared=True, device="cpu")
+    assert ladder.axes.tolist() == [0] * 11 + [1] * 11 + [2] * 10 and math.isclose(float(ladder.freqs[31]), 50.0 ** (-31 / 32), rel_tol=1e-6)
+    assert rotary_plan(torch.ones(4), torch.tensor([0, 1, 0, 1]), device="cpu").n_axes == 2
+    where = grid_positions(2, 3, device="cpu")
+    assert where.shape == (6, 2) and torch.allclose(where[1], torch.tensor([-0.5, 0.0])) and torch.allclose(where[5], torch.tensor([0.5, 2 / 3]))
+    for bad in (lambda: rotary_plan([1.0], [0, 1], device="cpu"), lambda: rotary_plan([], [], device="cpu"), lambda: rotary_plan([1.0], [-1], device="cpu"),
+                lambda: rotary_plan([1.0], [0.5], device="cpu"), lambda: rotary_plan([float("inf")], [0], device="cpu"),
+                lambda: rotary_plan([1.0], [0], pairing="all", device="cpu"), lambda: axial_plan(63, device="cpu"),
+                lambda: axial_plan(64, axes=2, shares=[10, 10], device="cpu"), lambda: axial_plan(4, axes=3, device="cpu")):
+        with pytest.raises(ValueError):
+            bad()
+
+
+def test_cpu_tensors_are_refused():
+    plan, q = axial_plan(64, device="cpu"), torch.zeros(1, 4, 2, 64)
+    with pytest.raises(ValueError, match="no CPU path"):
+        rotary(q, q, torch.zeros(4, 2), plan)
+
+
+def test_views_that_share_memory():
+    qkv = torch.zeros(2, 5, 3, 4, 8)
+    q, k, v = qkv.unbind(2)
+    assert _lib.disjoint(q, k) and _lib.disjoint(v, q) and not _lib.disjoint(q, q) and _lib.disjoint(q, torch.zeros_like(q))
+    flat = torch.zeros(2, 5, 8, 8)
+    assert _lib.disjoint(flat[:, :, :4], flat[:, :, 4:]) and not _lib.disjoint(flat[:, :, :5], flat[:, :, 4:]) and _lib.disjoint(flat[:, :, :6], flat[:, :, 6:])
+    assert _lib.disjoint(flat[0], flat[1]) and not _lib.disjoint(flat[:, 1:], flat[:, :4]) and _lib.disjoint(flat[:, 3:], flat[:, :3])
+    heads = torch.zeros(2, 3, 4, 5, 8)                       # [B, 3, H, N, D]
+    assert _lib.disjoint(heads[:, 0].transpose(1, 2), heads[:, 2].transpose(1, 2))
+    assert not _lib.disjoint(flat[:, ::2], flat[:, 0:3])
+    assert _lib.writable(q) and _lib.writable(heads.transpose(1, 3)) and not _lib.writable(flat[:1].expand(2, 5, 8, 8))
+    assert not _lib.writable(torch.zeros(20).as_strided((3, 8), (4, 1))) and _lib.same_view(q, qkv[:, :, 0]) and not _lib.same_view(q, k)
+
+
+def test_entry_point_refusals():
+    import ctypes
+    lib, A = _lib.load(), 0x7F0000000000
+
+    def call(heads=2, x=A, y=A, n=1, B=1, N=4, D=64, pairs=32, pairing=0, prefix=0, pos=A, pd=2, axes=2, freqs=A, ax=A, dtype=0):
+        t = (_lib.RotaryTensor * 2)()
+        t[0].x, t[0].y, t[0].heads = x, y, heads
+        return lib.fbb_rotary(ctypes.cast(t, ctypes.POINTER(_lib.RotaryTensor)), n, B, N, D, pairs, pairing, prefix, pos, pd, axes, 0, 2, 1, freqs, ax, 0, dtype, None)
+
+    assert call(x=None) == call(y=None) == call(freqs=None) == call(ax=None) == call(pos=None) == -1
+    assert call(heads=0) == call(n=3) == call(D=1026) == call(pairs=33) == call(pairs=0) == call(axes=0) == call(prefix=-1) == call(N=-1) == -2
+    assert call(B=1 << 20, N=1 << 20) == -2
+    assert call(x=A + 1) == call(y=A + 2, dtype=2) == call(pos=A + 4, pd=1) == -3
+    assert call(pairing=2) == call(pd=3) == call(dtype=4) == -4
+    assert call(B=0, x=None) == call(N=0, pos=None) == 0
