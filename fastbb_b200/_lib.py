@@ -134,7 +134,8 @@ def check(status):
 
 def stream_ptr(device=None):
     """cudaStream_t of torch's current stream on `device` as an integer (0 = legacy default stream)."""
-    return torch.cuda.current_stream(device).cuda_stream
+    index = device.index if device is not None else None
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
 def ptr(t):

@@ -19,6 +19,7 @@ namespace fbb {
 constexpr int kRotaryThreads = 256;
 constexpr int kRotaryUnroll = 4;
 constexpr int kRotaryTableEntries = 2048;  // (cos, sin) pairs of a CTA: 16 KB of shared memory
+constexpr int kRotaryMaxTokens = 64;       // of a CTA
 
 struct RotaryTensor {
     const char* x;
@@ -90,107 +91,146 @@ __device__ __forceinline__ T rotary_round(float v) {
     else return v;
 }
 
+// Where a token's heads begin in the two tensors; tensor 1's are heads heads0, heads0 + 1, ... of a row.
+struct RotaryRow {
+    const char* x[2];
+    char* y[2];
+};
+
 // HALF: pairing. VEC: 16-byte accesses; the scalar form (columns one by one) takes every size and stride that is not a multiple of
 // 16 bytes. A vector item of the half pairing is the two vectors at columns 8c and P + 8c, of the other pairing one vector; what is
 // left of a head (columns from 2P on) are plain copies behind them.
 template <typename T, bool HALF, bool VEC>
 __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryArgs a) {
     __shared__ __align__(16) float2 s_turn[kRotaryTableEntries];
+    __shared__ RotaryRow s_row[kRotaryMaxTokens];
+    __shared__ int s_pass[kRotaryMaxTokens];  // a row without a position
     grid_dependency_wait();
     grid_launch_dependents();
     const int64_t token0 = (int64_t)blockIdx.x * a.tokens_per_cta;
     const int count = (int)min((int64_t)a.tokens_per_cta, a.tokens - token0);
+    constexpr int E = VEC ? 16 / (int)sizeof(T) : 1;
+    const int turned = VEC ? (HALF ? a.P / E : 2 * a.P / E) : a.P;  // items of a head that turn; the others copy
+    const int64_t second = HALF ? (int64_t)a.P * (int)sizeof(T) : (int64_t)sizeof(T);
+    // A thread keeps its item of a head and walks the CTA's (token, head) rows in steps of `step`: no divisions on the way.
+    const int lanes = min(a.per_head, kRotaryThreads), step = kRotaryThreads / lanes;
+    const int lane = (int)threadIdx.x % lanes, row0 = (int)threadIdx.x / lanes;
+    for (int tok = threadIdx.x; tok < count; tok += kRotaryThreads) {
+        const uint32_t at = (uint32_t)token0 + (uint32_t)tok, b = at / (uint32_t)a.N, n = at - b * (uint32_t)a.N;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const RotaryTensor& t = a.t[i];
+            s_row[tok].x[i] = t.x + b * t.x_sb + n * t.x_sn - (i == 1 ? a.heads0 * t.x_sh : 0);
+            s_row[tok].y[i] = t.y + b * t.y_sb + n * t.y_sn - (i == 1 ? a.heads0 * t.y_sh : 0);
+        }
+        s_pass[tok] = (int)n < a.n_prefix;
+    }
+    __syncthreads();
+
+    struct Item {
+        uint4 u, w;
+        T su, sw;
+        char* dst;
+        int entry;  // first table entry, -1: copy, -2: beyond the CTA's rows
+    };
+    int c = lane, tok, head, first;
+    bool turn, two;
+    int64_t col;
+    auto begin = [&]() {  // the rows of item c from the first on
+        turn = c < turned;
+        two = turn && (HALF || !VEC);
+        col = (int64_t)(HALF || !turn ? (turn ? c * E : 2 * a.P + (c - turned) * E) : c * (VEC ? E : 2)) * (int)sizeof(T);
+        first = VEC && !HALF ? c * (E / 2) : c * E;  // of the item's table entries
+        tok = row0 / a.heads, head = row0 - tok * a.heads;
+        if (row0 >= step || c >= a.per_head) tok = count;
+    };
+    const int64_t x_sh0 = a.t[0].x_sh, x_sh1 = a.t[1].x_sh, y_sh0 = a.t[0].y_sh, y_sh1 = a.t[1].y_sh;
+    auto load = [&](Item& it) {
+        it.entry = -2;
+        if (tok >= count) return;
+        const bool other = head >= a.heads0;
+        const char* src = s_row[tok].x[other] + head * (other ? x_sh1 : x_sh0) + col;
+        it.dst = s_row[tok].y[other] + head * (other ? y_sh1 : y_sh0) + col;
+        it.entry = turn && !s_pass[tok] ? tok * a.P + first : -1;
+        if constexpr (VEC) {
+            it.u = *reinterpret_cast<const uint4*>(src);
+            if (two) it.w = *reinterpret_cast<const uint4*>(src + second);
+        } else {
+            it.su = *reinterpret_cast<const T*>(src);
+            if (two) it.sw = *reinterpret_cast<const T*>(src + second);
+        }
+        for (head += step; head >= a.heads; head -= a.heads) ++tok;
+    };
+    auto finish = [&](Item& it) {
+        if (it.entry == -2) return;
+        if constexpr (VEC) {
+            if (it.entry >= 0) {
+                float x[E], y[E];
+                rotary_unpack<T>(it.u, x);
+                if constexpr (HALF) {
+                    rotary_unpack<T>(it.w, y);
+#pragma unroll
+                    for (int e = 0; e < E; e += 2) {
+                        const float4 t = *reinterpret_cast<const float4*>(s_turn + it.entry + e);
+                        const float x0 = x[e], x1 = x[e + 1];
+                        x[e] = fmaf(x0, t.x, -y[e] * t.y), y[e] = fmaf(y[e], t.x, x0 * t.y);
+                        x[e + 1] = fmaf(x1, t.z, -y[e + 1] * t.w), y[e + 1] = fmaf(y[e + 1], t.z, x1 * t.w);
+                    }
+                    it.w = rotary_pack<T>(y);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < E; e += 4) {
+                        const float4 t = *reinterpret_cast<const float4*>(s_turn + it.entry + e / 2);
+                        const float x0 = x[e], x2 = x[e + 2];
+                        x[e] = fmaf(x0, t.x, -x[e + 1] * t.y), x[e + 1] = fmaf(x[e + 1], t.x, x0 * t.y);
+                        x[e + 2] = fmaf(x2, t.z, -x[e + 3] * t.w), x[e + 3] = fmaf(x[e + 3], t.z, x2 * t.w);
+                    }
+                }
+                it.u = rotary_pack<T>(x);
+            }
+            *reinterpret_cast<uint4*>(it.dst) = it.u;
+            if (two) *reinterpret_cast<uint4*>(it.dst + second) = it.w;
+        } else {
+            if (it.entry >= 0) {
+                const float x = rotary_value<T>(it.su), y = rotary_value<T>(it.sw);
+                const float2 t = s_turn[it.entry];
+                it.su = rotary_round<T>(fmaf(x, t.x, -y * t.y));
+                it.sw = rotary_round<T>(fmaf(y, t.x, x * t.y));
+            }
+            *reinterpret_cast<T*>(it.dst) = it.su;
+            if (two) *reinterpret_cast<T*>(it.dst + second) = it.sw;
+        }
+    };
+
+    // The first rows are on their way while the table is worked out.
+    Item items[kRotaryUnroll];
+    begin();
+#pragma unroll
+    for (int j = 0; j < kRotaryUnroll; ++j) load(items[j]);
     for (int i = threadIdx.x; i < count * a.P; i += kRotaryThreads) {
         const int tok = i / a.P, p = i - tok * a.P;
-        const int64_t b = (token0 + tok) / a.N;
-        const int n = (int)(token0 + tok - b * a.N) - a.n_prefix;
+        const uint32_t at = (uint32_t)token0 + (uint32_t)tok, b = at / (uint32_t)a.N;
+        const int n = (int)(at - b * (uint32_t)a.N) - a.n_prefix;
         float2 turn = make_float2(1.f, 0.f);
         if (n >= 0) {
             const int axis = min(max(a.axes[p], 0), a.n_axes - 1);
-            const double turns = rotary_position(a, b * a.p_sb + n * a.p_sn + axis * a.p_sa) * (double)a.freqs[p] * 0.15915494309189533577;
+            const double turns = rotary_position(a, (int64_t)b * a.p_sb + n * a.p_sn + axis * a.p_sa) * (double)a.freqs[p] * 0.15915494309189533577;
             sincospif(2.f * (float)(turns - rint(turns)), &turn.y, &turn.x);
             turn.y *= a.sign;
         }
         s_turn[i] = turn;
     }
     __syncthreads();
-
-    constexpr int E = VEC ? 16 / (int)sizeof(T) : 1;
-    const int per_token = a.heads * a.per_head;
-    const int items = count * per_token;
-    const int turned = VEC ? (HALF ? a.P / E : 2 * a.P / E) : a.P;  // items of a head that turn; the others copy
-    for (int i0 = threadIdx.x; i0 < items; i0 += kRotaryThreads * kRotaryUnroll) {
-        uint4 u[kRotaryUnroll], w[kRotaryUnroll];
-        T su[kRotaryUnroll], sw[kRotaryUnroll];
-        char* dst[kRotaryUnroll];
-        int entry[kRotaryUnroll];  // first table entry; -1: one vector (column) to copy, -2: two
+    for (;;) {
 #pragma unroll
-        for (int j = 0; j < kRotaryUnroll; ++j) {
-            const int i = i0 + j * kRotaryThreads;
-            if (i >= items) continue;
-            const int tok = i / per_token, r = i - tok * per_token;
-            int head = r / a.per_head;
-            const int c = r - head * a.per_head;
-            const int64_t b = (token0 + tok) / a.N;
-            const int n = (int)(token0 + tok - b * a.N);
-            const RotaryTensor& t = a.t[head >= a.heads0 ? 1 : 0];
-            if (head >= a.heads0) head -= a.heads0;
-            const bool turn = c < turned;
-            const int col = HALF || !turn ? (turn ? c * E : 2 * a.P + (c - turned) * E) : c * (VEC ? E : 2);
-            const char* src = t.x + b * t.x_sb + n * t.x_sn + head * t.x_sh + (int64_t)col * (int)sizeof(T);
-            dst[j] = t.y + b * t.y_sb + n * t.y_sn + head * t.y_sh + (int64_t)col * (int)sizeof(T);
-            const bool two = turn && (HALF || !VEC);
-            entry[j] = (turn && n >= a.n_prefix) ? tok * a.P + (VEC && !HALF ? c * (E / 2) : c * E) : (two ? -2 : -1);
-            const int64_t second = HALF ? (int64_t)a.P * (int)sizeof(T) : (int64_t)sizeof(T);
-            if constexpr (VEC) {
-                u[j] = *reinterpret_cast<const uint4*>(src);
-                if (two) w[j] = *reinterpret_cast<const uint4*>(src + second);
-            } else {
-                su[j] = *reinterpret_cast<const T*>(src);
-                if (two) sw[j] = *reinterpret_cast<const T*>(src + second);
-            }
+        for (int j = 0; j < kRotaryUnroll; ++j) finish(items[j]);
+        if (tok >= count) {
+            c += lanes;
+            if (c >= a.per_head) break;
+            begin();
         }
 #pragma unroll
-        for (int j = 0; j < kRotaryUnroll; ++j) {
-            if (i0 + j * kRotaryThreads >= items) continue;
-            const int64_t second = HALF ? (int64_t)a.P * (int)sizeof(T) : (int64_t)sizeof(T);
-            if constexpr (VEC) {
-                if (entry[j] >= 0) {
-                    float x[E], y[E];
-                    rotary_unpack<T>(u[j], x);
-                    if constexpr (HALF) {
-                        rotary_unpack<T>(w[j], y);
-#pragma unroll
-                        for (int e = 0; e < E; e += 2) {
-                            const float4 t = *reinterpret_cast<const float4*>(s_turn + entry[j] + e);
-                            const float x0 = x[e], x1 = x[e + 1];
-                            x[e] = fmaf(x0, t.x, -y[e] * t.y), y[e] = fmaf(y[e], t.x, x0 * t.y);
-                            x[e + 1] = fmaf(x1, t.z, -y[e + 1] * t.w), y[e + 1] = fmaf(y[e + 1], t.z, x1 * t.w);
-                        }
-                        w[j] = rotary_pack<T>(y);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < E; e += 2) {
-                            const float2 t = s_turn[entry[j] + e / 2];
-                            const float x0 = x[e];
-                            x[e] = fmaf(x0, t.x, -x[e + 1] * t.y), x[e + 1] = fmaf(x[e + 1], t.x, x0 * t.y);
-                        }
-                    }
-                    u[j] = rotary_pack<T>(x);
-                }
-                *reinterpret_cast<uint4*>(dst[j]) = u[j];
-                if (HALF && entry[j] != -1) *reinterpret_cast<uint4*>(dst[j] + second) = w[j];
-            } else {
-                if (entry[j] >= 0) {
-                    const float x = rotary_value<T>(su[j]), y = rotary_value<T>(sw[j]);
-                    const float2 t = s_turn[entry[j]];
-                    su[j] = rotary_round<T>(fmaf(x, t.x, -y * t.y));
-                    sw[j] = rotary_round<T>(fmaf(y, t.x, x * t.y));
-                }
-                *reinterpret_cast<T*>(dst[j]) = su[j];
-                if (entry[j] != -1) *reinterpret_cast<T*>(dst[j] + second) = sw[j];
-            }
-        }
+        for (int j = 0; j < kRotaryUnroll; ++j) load(items[j]);
     }
 }
 
@@ -200,9 +240,9 @@ static cudaError_t rotary_launch(RotaryArgs a, bool half, bool vec, cudaStream_t
     a.per_head = (vec ? (half ? a.P / E : 2 * a.P / E) : a.P) + (a.D - 2 * a.P) / E;
     // As many tokens a CTA as give each thread kRotaryUnroll items, fewer where that leaves SMs without two CTAs.
     const int per_token = a.heads * a.per_head;
-    int64_t per_cta = (kRotaryThreads * kRotaryUnroll + per_token - 1) / per_token;
+    int64_t per_cta = kRotaryThreads * kRotaryUnroll / per_token;
     per_cta = min(per_cta, (a.tokens + 2 * num_sms() - 1) / (2 * num_sms()));
-    per_cta = min(per_cta, (int64_t)(kRotaryTableEntries / max(a.P, 1)));
+    per_cta = min(per_cta, (int64_t)min(kRotaryTableEntries / a.P, kRotaryMaxTokens));
     a.tokens_per_cta = (int)max(per_cta, (int64_t)1);
     const dim3 grid((unsigned)((a.tokens + a.tokens_per_cta - 1) / a.tokens_per_cta));
     auto kern = half ? (vec ? rotary_kernel<T, true, true> : rotary_kernel<T, true, false>) : (vec ? rotary_kernel<T, false, true> : rotary_kernel<T, false, false>);

@@ -10,9 +10,6 @@ video, turned in one launch between the qkv projection and the attention.
 The reference has no counterpart: the models it speeds up add a learned position table to their tokens
 (fastbb/vit.py FastViT.tokens).
 """
-import collections
-import ctypes
-
 import torch
 
 from . import _lib
@@ -20,16 +17,24 @@ from . import _lib
 _PAIRING = {"half": 0, "pairs": 1}
 _POS_CODE = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
 
-RotaryPlan = collections.namedtuple("RotaryPlan", "freqs axes n_axes pairing")
-RotaryPlan.__doc__ = """What a model's layers share: freqs [pairs] fp32 and axes [pairs] int32 on the GPU (pair i turns by the position on
-axis axes[i] times freqs[i]), the number of axes, and how columns pair: "half" (i, i + pairs) or "pairs" (2i, 2i + 1)."""
+
+class RotaryPlan:
+    """What a model's layers share: freqs [pairs] fp32 and axes [pairs] int32 on the GPU (pair i turns by the position on axis axes[i]
+    times freqs[i]), the number of axes, and how columns pair: "half" (i, i + pairs) or "pairs" (2i, 2i + 1). Made by rotary_plan."""
+    __slots__ = ("freqs", "axes", "n_axes", "pairing", "pairs", "device")
+
+    def __init__(self, freqs, axes, n_axes, pairing):
+        if pairing not in _PAIRING:
+            raise ValueError(f"unsupported pairing: {pairing} (expected one of {tuple(_PAIRING)})")
+        if freqs.dtype != torch.float32 or axes.dtype != torch.int32 or freqs.device != axes.device or not (
+                freqs.dim() == axes.dim() == 1 and freqs.numel() == axes.numel() > 0 and freqs.is_contiguous() and axes.is_contiguous()) or n_axes < 1:
+            raise ValueError("freqs must be fp32 and axes int32 vectors of one length on one device, n_axes at least 1")
+        self.freqs, self.axes, self.n_axes, self.pairing, self.pairs, self.device = freqs, axes, n_axes, pairing, freqs.numel(), freqs.device
 
 
 def rotary_plan(freqs, axes, pairing="half", device="cuda"):
     """A RotaryPlan from any sequence (or CPU / GPU tensor) of frequencies in radians per unit of position and one of axis numbers, one
     of each per pair of columns: sections, interleaved axes and ladders of any kind are sequences. Reads GPU tensors back: make it once."""
-    if pairing not in _PAIRING:
-        raise ValueError(f"unsupported pairing: {pairing} (expected one of {tuple(_PAIRING)})")
     freqs = torch.as_tensor(freqs, dtype=torch.float64).flatten().cpu()
     axes = torch.as_tensor(axes).flatten().cpu()
     if axes.is_floating_point() or axes.dtype == torch.bool:
@@ -75,56 +80,67 @@ def rotary(q, k, positions, plan, n_prefix=0, inverse=False, out=None):
     positions: [N - n_prefix, axes] for every sequence alike, or [B, N - n_prefix, axes]; int32, int64 or fp32.
     inverse: the transposed rotation, which undoes this one and takes gradients of (q', k') to gradients of (q, k).
     out: (q_out, k_out); each may be its own input (in place), otherwise it shares no memory with either input."""
-    inputs = [q] if k is None else [q, k]
-    for x in inputs:
-        if not (x.is_cuda and x.dim() == 4 and x.dtype in _lib.DTYPE_CODE and (x.stride(3) == 1 or x.shape[3] == 1)):
-            raise ValueError("rotary needs CUDA fp16, bf16 or fp32 [B, N, H, D] tensors with a contiguous last dim (there is no CPU path)")
-    B, N, H, D = q.shape
-    if k is not None and (k.device != q.device or k.dtype != q.dtype or k.shape[:2] != q.shape[:2] or k.shape[3] != D):
-        raise ValueError("k must have q's batch, tokens, columns, dtype and device")
-    if min(x.shape[2] for x in inputs) < 1 or D > 1024:
+    shape, device, dtype = q.shape, q.device, q.dtype
+    code = _lib.DTYPE_CODE.get(dtype)
+    if not q.is_cuda or code is None or len(shape) != 4:
+        raise ValueError("rotary needs CUDA fp16, bf16 or fp32 [B, N, H, D] tensors (there is no CPU path)")
+    B, N, H, D = shape
+    q_strides, heads = q.stride(), H
+    if k is not None:
+        k_shape, k_strides = k.shape, k.stride()
+        if k.device != device or k.dtype != dtype or len(k_shape) != 4 or k_shape[0] != B or k_shape[1] != N or k_shape[3] != D:
+            raise ValueError("k must have q's batch, tokens, columns, dtype and device")
+        heads = min(H, k_shape[2])
+    if D > 1 and (q_strides[3] != 1 or (k is not None and k_strides[3] != 1)):
+        raise ValueError("rotary needs tensors with a contiguous last dim")
+    if heads < 1 or D > 1024:
         raise ValueError("rotary needs at least one head and at most 1024 columns")
-    pairs = plan.freqs.numel()
-    if plan.freqs.device != q.device or plan.axes.device != q.device:
-        raise ValueError(f"the plan is on {plan.freqs.device}, the tensors on {q.device}")
-    if plan.freqs.dtype != torch.float32 or plan.axes.dtype != torch.int32 or plan.axes.numel() != pairs or plan.pairing not in _PAIRING:
-        raise ValueError("plan must come from rotary_plan or axial_plan")
+    if plan.device != device:
+        raise ValueError(f"the plan is on {plan.device}, the tensors on {device}")
+    pairs, n_axes = plan.pairs, plan.n_axes
     if 2 * pairs > D:
         raise ValueError(f"the plan turns {2 * pairs} columns, a head has {D}")
     if n_prefix < 0 or n_prefix > N:
         raise ValueError(f"n_prefix must be from 0 to {N}")
-    if positions.device != q.device or positions.dtype not in _POS_CODE:
+    pos_code, pos_shape, pos_strides = _POS_CODE.get(positions.dtype), positions.shape, positions.stride()
+    if pos_code is None or positions.device != device:
         raise ValueError("positions must be int32, int64 or fp32 on the tensors' device")
-    if positions.shape not in ((N - n_prefix, plan.n_axes), (B, N - n_prefix, plan.n_axes)):
-        raise ValueError(f"positions must be [{N - n_prefix}, {plan.n_axes}] or [{B}, {N - n_prefix}, {plan.n_axes}], got {tuple(positions.shape)}")
+    if pos_shape != (N - n_prefix, n_axes) and pos_shape != (B, N - n_prefix, n_axes):
+        raise ValueError(f"positions must be [{N - n_prefix}, {n_axes}] or [{B}, {N - n_prefix}, {n_axes}], got {tuple(pos_shape)}")
+    if len(pos_shape) == 2:
+        pos_strides = (0, *pos_strides)
     if out is None:
-        outs = [torch.empty(x.shape, device=x.device, dtype=x.dtype) for x in inputs]
+        result = torch.empty(shape, device=device, dtype=dtype), torch.empty(k_shape, device=device, dtype=dtype) if k is not None else None
     else:
-        outs = list(out)
-        if len(outs) == 2 and k is None and outs[1] is None:
-            outs.pop()
-        if len(outs) != len(inputs):
-            raise ValueError("out must be a pair (q_out, k_out)")
-        for i, y in enumerate(outs):
-            if y.shape != inputs[i].shape or y.dtype != q.dtype or y.device != q.device or (y.stride(3) != 1 and D > 1) or not _lib.writable(y):
-                raise ValueError("out must match the inputs' shapes, dtype and device, with a contiguous last dim and no element twice")
-            if not all(_lib.disjoint(y, x) or (i == j and _lib.same_view(y, x)) for j, x in enumerate(inputs)):
-                raise ValueError("out must be its own input or share no memory with the inputs")
-        if len(outs) == 2 and not _lib.disjoint(*outs):
-            raise ValueError("the two outputs share memory")
-    result = (outs[0], outs[1] if k is not None else None)
+        result = _checked(out, q, k)
     if B == 0 or N == 0:
         return result
+    y, y_strides = result[0], result[0].stride()
     tensors = (_lib.RotaryTensor * 2)()
-    for t, x, y in zip(tensors, inputs, outs):
-        t.x, t.y, t.heads = x.data_ptr(), y.data_ptr(), x.shape[2]
-        t.x_sb, t.x_sn, t.x_sh = x.stride()[:3]
-        t.y_sb, t.y_sn, t.y_sh = y.stride()[:3]
-    sb, sn, sa = (0, *positions.stride()) if positions.dim() == 2 else positions.stride()
-    with _lib.on(q.device):
+    tensors[0] = (q.data_ptr(), y.data_ptr(), H, *q_strides[:3], *y_strides[:3])
+    if k is not None:
+        y, y_strides = result[1], result[1].stride()
+        tensors[1] = (k.data_ptr(), y.data_ptr(), k_shape[2], *k_strides[:3], *y_strides[:3])
+    with _lib.on(device):
         _lib.check(_lib.load().fbb_rotary(
-            ctypes.cast(tensors, ctypes.POINTER(_lib.RotaryTensor)), len(inputs), B, N, D, pairs, _PAIRING[plan.pairing], n_prefix, positions.data_ptr(),
-            _POS_CODE[positions.dtype], plan.n_axes, sb, sn, sa, plan.freqs.data_ptr(), plan.axes.data_ptr(), 1 if inverse else 0,
-            _lib.DTYPE_CODE[q.dtype], _lib.stream_ptr(q.device)))
+            tensors, 1 if k is None else 2, B, N, D, pairs, _PAIRING[plan.pairing], n_prefix, positions.data_ptr(), pos_code, n_axes, *pos_strides,
+            plan.freqs.data_ptr(), plan.axes.data_ptr(), 1 if inverse else 0, code, _lib.stream_ptr(device)))
     _lib.launched()
     return result
+
+
+def _checked(out, q, k):
+    """The caller's pair of outputs, refused where two threads could meet on an element."""
+    inputs, outs = [q] if k is None else [q, k], list(out)
+    if len(outs) == 2 and k is None and outs[1] is None:
+        outs.pop()
+    if len(outs) != len(inputs):
+        raise ValueError("out must be a pair (q_out, k_out)")
+    for i, y in enumerate(outs):
+        if y.shape != inputs[i].shape or y.dtype != q.dtype or y.device != q.device or (y.stride(3) != 1 and y.shape[3] > 1) or not _lib.writable(y):
+            raise ValueError("out must match the inputs' shapes, dtype and device, with a contiguous last dim and no element twice")
+        if not all(_lib.disjoint(y, x) or (i == j and _lib.same_view(y, x)) for j, x in enumerate(inputs)):
+            raise ValueError("out must be its own input or share no memory with the inputs")
+    if len(outs) == 2 and not _lib.disjoint(*outs):
+        raise ValueError("the two outputs share memory")
+    return outs[0], outs[1] if k is not None else None
