@@ -278,6 +278,33 @@ int fbb_linear_layernorm_f16(const void* A, const void* W, void* C, const void* 
                                    counter, (cudaStream_t)stream);
 }
 
+int64_t fbb_diff64_workspace_bytes(int B, int Nq, int Nk, int H) { return diff64_workspace_bytes(B, Nq, Nk, H); }
+int fbb_diff64_launches(int B, int Nq, int Nk, int H) { return diff64_launches(B, Nq, Nk, H); }
+
+int fbb_diff64_f16(const void* q, const void* k, const void* v, void* o, int B, int Nq, int Nk, int H, int Hk, int64_t q_sb, int64_t q_sn,
+                   int64_t q_sh, int64_t k_sb, int64_t k_sn, int64_t k_sh, int64_t v_sb, int64_t v_sn, int64_t v_sh, int64_t o_sb, int64_t o_sn,
+                   int64_t o_sh, const float* lam, int64_t lam_sb, int64_t lam_sn, int64_t lam_sh, const void* weight, int weight_dtype, float eps,
+                   float out_scale, float scale, const int* lengths, void* workspace, int64_t workspace_bytes, void* stream) {
+    if (B < 0 || Nq < 0 || Nk < 0 || H <= 0 || Hk <= 0 || H % Hk != 0 || (int64_t)B * H > 0x7FFFFFFFll || H > 65535)
+        return fail(FBB_ERR_SHAPE, "diff64: bad B/Nq/Nk/H/Hk (%d, %d, %d, %d, %d)", B, Nq, Nk, H, Hk);
+    if (weight != nullptr && weight_dtype != FBB_DTYPE_F16 && weight_dtype != FBB_DTYPE_F32) return fail(FBB_ERR_ENUM, "diff64: weight dtype %d", weight_dtype);
+    if (!(scale > 0.f) || !(eps >= 0.f)) return fail(FBB_ERR_SHAPE, "diff64: scale must be > 0 and eps >= 0");
+    if (B == 0 || Nq == 0) return FBB_OK;
+    if (q == nullptr || o == nullptr || lam == nullptr || (Nk > 0 && (k == nullptr || v == nullptr))) return fail(FBB_ERR_NULL, "diff64: q, k, v, o or lam is null");
+    const int64_t qs[3] = {q_sb, q_sn, q_sh}, ks[3] = {k_sb, k_sn, k_sh}, vs[3] = {v_sb, v_sn, v_sh}, os[3] = {o_sb, o_sn, o_sh};
+    const int64_t ls[3] = {lam_sb, lam_sn, lam_sh};
+    const int sizes[4][3] = {{B, Nq, 2 * H}, {B, Nk, 2 * Hk}, {B, Nk, Hk}, {B, Nq, H}};
+    const int64_t* strides[4] = {qs, ks, vs, os};
+    for (int i = 0; i < 4; ++i)
+        for (int d = 0; d < 3; ++d)
+            if (sizes[i][d] > 1 && ((strides[i][d] & 7) != 0 || strides[i][d] <= 0))
+                return fail(FBB_ERR_ALIGN, "diff64: strides must be positive multiples of 8 elements");
+    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !aligned16(workspace))
+        return fail(FBB_ERR_ALIGN, "diff64: q, k, v, o and workspace must be 16-byte aligned");
+    return launch_diff64(q, k, v, o, B, Nq, Nk, H, Hk, qs, ks, vs, os, lam, ls, weight, weight_dtype, eps, out_scale, scale, lengths, workspace,
+                         workspace_bytes, (cudaStream_t)stream);
+}
+
 int fbb_rotary(const fbb_rotary_tensor* tensors, int n_tensors, int B, int N, int D, int pairs, int pairing, int n_prefix, const void* positions,
                int pos_dtype, int n_axes, int64_t p_sb, int64_t p_sn, int64_t p_sa, const float* freqs, const int* axes, int inverse, int dtype,
                void* stream) {

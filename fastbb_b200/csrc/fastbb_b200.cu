@@ -3,6 +3,7 @@
 #include "layernorm.cu"
 #include "gemm.cu"
 #include "flash64.cu"
+#include "diff64.cu"
 #include "rotary.cu"
 #include "block.cu"
 #include "api.cu"

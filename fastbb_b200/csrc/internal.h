@@ -102,6 +102,13 @@ int flash64_static_workspace(void** ptr, int64_t* bytes, cudaStream_t stream);
 int64_t flash64_workspace_bytes_for(int B, int N, int H);
 int flash64_launches(int B, int N, int H, bool has_workspace);
 
+// Differential attention (diff64.cu). Strides in elements, {batch, token, head} each; ls: lam's.
+int64_t diff64_workspace_bytes(int B, int Nq, int Nk, int H);
+int diff64_launches(int B, int Nq, int Nk, int H);
+int launch_diff64(const void* q, const void* k, const void* v, void* o, int B, int Nq, int Nk, int H, int Hk, const int64_t* qs, const int64_t* ks,
+                  const int64_t* vs, const int64_t* os, const float* lam, const int64_t* ls, const void* weight, int weight_dtype, float eps,
+                  float out_scale, float scale, const int* lengths, void* ws, int64_t ws_bytes, cudaStream_t stream);
+
 int launch_rotary(const fbb_rotary_tensor* t, int n_tensors, int B, int N, int D, int pairs, int pairing, int n_prefix, const void* pos, int pos_dtype,
                   int n_axes, int64_t p_sb, int64_t p_sn, int64_t p_sa, const float* freqs, const int* axes, int inverse, int dtype, cudaStream_t stream);
 

@@ -192,6 +192,26 @@ int fbb_flash64_f16_static(const void* q, const void* k, const void* v, void* o,
                            int64_t q_sh, int64_t k_sb, int64_t k_sn, int64_t k_sh, int64_t v_sb, int64_t v_sn, int64_t v_sh,
                            int64_t o_sb, int64_t o_sn, int64_t o_sh, float scale, int variant, void* stream);
 
+/* ---- differential attention -----------------------------------------------------------------------------------------------
+ * o = softmax(scale q1 k1^T) v - lam softmax(scale q2 k2^T) v: two maps of head dimension 64 over the same values of 128 columns;
+ * with a weight followed by the norm of every row of 128, o * weight / sqrt(mean(o^2) + eps); both times out_scale. No counterpart
+ * in the reference; it stands beside fbb_flash64_f16, with one launch (and one pass over v) for what takes four of that.
+ * q: [B, Nq, 2H, 64], head h's maps are heads 2h and 2h + 1; k: [B, Nk, 2Hk, 64]; v: [B, Nk, Hk, 128]; o: [B, Nq, H, 128]; fp16, last
+ * dimension contiguous, the other strides (batch, token, head) multiples of 8 elements, positive where the dimension has more than one
+ * element; Hk divides H (query heads in a row share a key head). lam: fp32 [B, Nq, H] with strides of its own (0: broadcast).
+ * weight: [128] of weight_dtype (fp16 or fp32) or null. lengths: int32 [B] or null; keys from lengths[b] on are not seen, whatever k and
+ * v hold there (a number below 0 counts as 0, beyond Nk as Nk); without any key a row of o is 0. scale > 0.
+ * Scores, maxima, sums and outputs are fp32; the probabilities are rounded to fp16 for the second product, relative to a maximum that
+ * is at most 2^8 too small.
+ * workspace: fbb_diff64_workspace_bytes() of 16-byte aligned device memory (0 bytes where the keys are not split), overwritten
+ * freely; calls that may overlap in time need different ones. fbb_diff64_launches: kernels a call enqueues (1, or 2 with split keys). */
+int64_t fbb_diff64_workspace_bytes(int B, int Nq, int Nk, int H);
+int fbb_diff64_launches(int B, int Nq, int Nk, int H);
+int fbb_diff64_f16(const void* q, const void* k, const void* v, void* o, int B, int Nq, int Nk, int H, int Hk, int64_t q_sb, int64_t q_sn,
+                   int64_t q_sh, int64_t k_sb, int64_t k_sn, int64_t k_sh, int64_t v_sb, int64_t v_sn, int64_t v_sh, int64_t o_sb, int64_t o_sn,
+                   int64_t o_sh, const float* lam, int64_t lam_sb, int64_t lam_sn, int64_t lam_sh, const void* weight, int weight_dtype, float eps,
+                   float out_scale, float scale, const int* lengths, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* ---- rotary positions ---------------------------------------------------------------------------------------------------
  * Queries and keys turned by the positions of their tokens on one or several axes, one launch for both. No counterpart in the
  * reference (its models have learned position tables); it stands between fbb_linear_f16 (qkv) and fbb_flash64_f16.

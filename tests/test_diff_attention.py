@@ -1,0 +1,240 @@
+"""diff_attention(): against the definition in 64 bits over sizes, head groups, layouts, key lengths and peaked rows; refusals.
+
+Tolerance, per element. Probabilities are rounded to fp16 ahead of the second product: half a step, 2^-11 relative, and half of fp16's
+smallest step, 2^-25, for those that small (relative to a maximum whose own probability is at least 1). Scores are fp32 sums of 64 exact
+products, off by less than 64 * 2^-24 * sum |q k| * scale, which is what the exponent and so the probability is off by relatively
+(times 1.45, with 2^-21 for the exponential and the fp32 sums): with these, map t's output is off by at most
+  d_t = (2^-11 + e_t) A_t + 2^-25 S / l_t,   A_t = softmax-weighted |v|, S = sum |v|, l_t = sum of exp(score - maximum),  e_t the exponents'.
+o is off by d = d_1 + |lam| d_2 (+ 2^-22 of |o_1| + |lam o_2| for the fp32 end). The norm y = o r w s, r = (mean o^2 + eps)^-1/2, is off by
+|w s| r (d + |o| r rms(d)) to first order; a fifth more covers the second where r rms(d) < 0.1, which is checked. The result is rounded
+to fp16: 2^-11 of it, or 2^-25."""
+import pytest
+import torch
+
+from fastbb_b200 import _lib
+from fastbb_b200.diff_attention import diff_attention
+
+
+def reference(q, k, v, lam, weight=None, eps=1e-5, out_scale=1.0, scale=0.125, lengths=None):
+    """(o, room) in 64 bits, room the tolerance."""
+    B, Nq, H2, _ = q.shape
+    H, Hk, Nk = H2 // 2, v.shape[2], k.shape[1]
+    lam = lam.double().expand(B, Nq, H)
+    o = torch.zeros(B, Nq, H, 128, dtype=torch.float64, device=q.device)
+    d = torch.zeros_like(o)
+    for b in range(B):
+        n = Nk if lengths is None else min(max(int(lengths[b]), 0), Nk)
+        for h in range(H if n else 0):
+            vv = v[b, :n, h * Hk // H].double()
+            for t in range(2):
+                kk = k[b, :n, 2 * (h * Hk // H) + t].double()
+                for lo in range(0, Nq, 1024):
+                    qq = q[b, lo:lo + 1024, 2 * h + t].double()
+                    s = qq @ kk.t() * scale
+                    off = (qq.abs() @ kk.abs().t()).amax(-1, keepdim=True) * scale * 64 * 2.0 ** -24 * 1.45
+                    p = torch.exp(s - s.amax(-1, keepdim=True))
+                    l = p.sum(-1, keepdim=True)
+                    x = p @ vv / l
+                    dx = (2.0 ** -11 + 2 * off + 2.0 ** -21) * (p @ vv.abs() / l) + 2.0 ** -25 * vv.abs().sum(0) / l + 2.0 ** -22 * x.abs()
+                    f = 1.0 if t == 0 else lam[b, lo:lo + 1024, h, None]
+                    o[b, lo:lo + 1024, h] += x if t == 0 else -f * x
+                    d[b, lo:lo + 1024, h] += dx if t == 0 else f.abs() * dx
+    if weight is not None:
+        r = (o.square().mean(-1, keepdim=True) + eps).rsqrt()
+        rms = d.square().mean(-1, keepdim=True).sqrt() * r
+        assert float(rms.max()) < 0.1
+        d = 1.2 * weight.double().abs() * r * (d + o.abs() * rms)
+        o = o * r * weight.double()
+    o, d = o * out_scale, d * abs(out_scale)
+    return o, d + o.abs() * 2.0 ** -11 + 2.0 ** -25
+
+
+def check(got, *args, **kw):
+    want, room = reference(*args, **kw)
+    over = (got.double() - want).abs() - room
+    assert bool((over <= 0).all()), f"{int((~(over <= 0)).sum())} of {over.numel()} off, worst by {float(over.max()):.3g}, room there {float(room.flatten()[over.argmax()]):.3g}"
+
+
+def make(B, Nq, Nk, H, Hk, g, lam="head", std=1.0):
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    lam = torch.rand({"one": (), "head": (H,), "token": (B, Nq, H), "row": (Nq, 1)}[lam], generator=g, device="cuda") * 0.8
+    return (rnd(B, Nq, 2 * H, 64) * std).half(), rnd(B, Nk, 2 * Hk, 64).half(), rnd(B, Nk, Hk, 128).half(), lam
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,Nq,Nk,H,Hk,lam,norm", [
+    (1, 1, 1, 1, 1, "one", False), (1, 1, 127, 2, 1, "head", True), (2, 3, 128, 1, 1, "token", True), (1, 16, 129, 3, 1, "head", False),
+    (2, 17, 64, 4, 2, "row", True), (1, 128, 128, 2, 2, "head", True), (1, 129, 257, 6, 6, "token", True), (2, 200, 300, 3, 3, "head", False),
+    (1, 257, 257, 6, 2, "head", True), (1, 1, 5000, 3, 3, "head", True), (3, 5, 2049, 2, 1, "token", True), (1, 40, 16385, 1, 1, "one", True),
+    (1, 500, 1500, 2, 2, "token", True), (9, 131, 384, 12, 4, "head", True), (1, 1041, 1041, 16, 16, "head", True), (2, 640, 7, 2, 2, "head", False)])
+def test_matches_the_definition_in_64_bits(B, Nq, Nk, H, Hk, lam, norm):
+    g = torch.Generator("cuda").manual_seed(Nq * 31 + Nk)
+    q, k, v, lam = make(B, Nq, Nk, H, Hk, g, lam)
+    weight = torch.randn(128, generator=g, device="cuda").mul_(0.2).add_(1)
+    weight = None if not norm else weight.half() if Nq % 2 else weight
+    out = diff_attention(q, k, v, lam, weight=weight, out_scale=0.8)
+    check(out, q, k, v, lam, weight=weight, out_scale=0.8)
+    assert torch.equal(out, diff_attention(q, k, v, lam, weight=weight, out_scale=0.8))  # the same bits again
+    assert _lib.device_status() == (0, 0, 0, 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Nq,Nk,lengths", [(5, 400, [400, 0, 1, 128, 129, 399]), (300, 300, [300, 127, 0, 256, 255, 64]), (1, 4000, [3999, 4000, 0, 17, 2048, 2049]),
+                                           (130, 129, [-3, 500, 129, 128, 65, 2])])
+@pytest.mark.parametrize("bad", [0.0, float("nan"), float("inf")])
+def test_keys_beyond_a_length_are_not_seen(Nq, Nk, lengths, bad):
+    g = torch.Generator("cuda").manual_seed(Nk)
+    q, k, v, lam = make(len(lengths), Nq, Nk, 2, 1, g, "token")
+    weight = torch.randn(128, generator=g, device="cuda").half()
+    for i, n in enumerate(lengths):
+        if bad and n < Nk:
+            k[i, max(n, 0):], v[i, max(n, 0):] = bad, -bad
+    n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    out = diff_attention(q, k, v, lam, weight=weight, key_lengths=n)
+    clean_k, clean_v = k.nan_to_num(0, 0, 0), v.nan_to_num(0, 0, 0)
+    check(out, q, clean_k, clean_v, lam, weight=weight, lengths=lengths)
+    for i, m in enumerate(lengths):
+        if m <= 0:
+            assert bool((out[i] == 0).all())
+    plain = diff_attention(q, k, v, lam, key_lengths=n, scale=0.3)
+    check(plain, q, clean_k, clean_v, lam, lengths=lengths, scale=0.3)
+
+
+@pytest.mark.gpu
+def test_no_keys_at_all():
+    g = torch.Generator("cuda").manual_seed(1)
+    q, k, v, lam = make(2, 5, 0, 2, 2, g)
+    out = torch.full((2, 5, 2, 128), float("nan"), device="cuda", dtype=torch.float16)
+    assert bool((diff_attention(q, k, v, lam, out=out) == 0).all())
+    assert diff_attention(q[:0], k[:0], v[:0], lam).shape == (0, 5, 2, 128) and diff_attention(q[:, :0], k, v, lam).shape == (2, 0, 2, 128)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Nq,Nk", [(150, 700), (2, 3000)])
+def test_maxima_that_rise_block_after_block(Nq, Nk):
+    """Keys aligned with the queries and growing along the sequence: every block exceeds the running maximum by far more than 2^8."""
+    g = torch.Generator("cuda").manual_seed(9)
+    q, k, v, lam = make(1, Nq, Nk, 2, 2, g)
+    q = (q * 0.2 + 1).half()
+    k = (k * 0.1 + torch.linspace(0, 20, Nk, device="cuda")[None, :, None, None]).half()
+    check(diff_attention(q, k, v, lam), q, k, v, lam)
+    check(diff_attention(q, k.flip(1), v, lam), q, k.flip(1), v, lam)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout", ["packed", "heads first", "wide"])
+def test_strided_views_and_a_strided_output(layout):
+    g = torch.Generator("cuda").manual_seed(4)
+    B, N, H = 2, 205, 3
+    if layout == "packed":
+        buf = torch.randn(B, N, 6 * H * 64, generator=g, device="cuda").half()
+        q, k, v = (t.view(B, N, -1, c) for t, c in zip(buf.split(2 * H * 64, -1), (64, 64, 128)))
+    elif layout == "heads first":
+        q, k = (torch.randn(B, 2 * H, N, 64, generator=g, device="cuda").half().transpose(1, 2) for _ in range(2))
+        v = torch.randn(B, H, N, 128, generator=g, device="cuda").half().transpose(1, 2)
+    else:
+        q, k = (torch.randn(2 * B, N, 2 * H, 72, generator=g, device="cuda").half()[::2, ..., 8:] for _ in range(2))
+        v = torch.randn(B, 2 * N, H, 128, generator=g, device="cuda").half()[:, 1::2]
+    lam = torch.rand(H, N, B, generator=g, device="cuda").permute(2, 1, 0)
+    frame = torch.full((B, N + 3, H + 1, 136), 7.0, device="cuda", dtype=torch.float16)
+    out = diff_attention(q, k, v, lam, out=frame[:, 1:N + 1, :H, :128])
+    check(out, q, k, v, lam)
+    out.fill_(7.0)
+    assert bool((frame == 7.0).all())  # nothing outside the rows was written
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits():
+    g = torch.Generator("cuda").manual_seed(5)
+    far = 2 ** 31 + 4096
+    store = torch.empty(far + 2 * 128 * 300, device="cuda", dtype=torch.float16)
+    q, k, v, lam = make(2, 70, 150, 1, 1, g)
+    kb = store.as_strided((2, 150, 2, 64), (far, 128, 64, 1))
+    vb = store.as_strided((2, 150, 1, 128), (far, 128, 128, 1), 128 * 150)
+    ob = torch.empty(far + 128 * 70, device="cuda", dtype=torch.float16).as_strided((2, 70, 1, 128), (far, 128, 128, 1))
+    kb.copy_(k)
+    vb.copy_(v)
+    check(diff_attention(q, kb, vb, lam, out=ob), q, k, v, lam)
+
+
+@pytest.mark.gpu
+def test_other_stream_and_graphs_that_live_side_by_side():
+    g = torch.Generator("cuda").manual_seed(6)
+    sets = [make(1, n, m, 4, 4, g) for n, m in ((3, 3000), (260, 260), (1, 6000))]
+    want = [diff_attention(*s) for s in sets]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = [diff_attention(*s) for s in sets]
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for s in sets:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            graphs.append((graph, diff_attention(*s)))
+    for _ in range(2):
+        for (graph, out), w in zip(graphs, want):
+            out.zero_()
+            graph.replay()
+    for o, (_, c), w in zip(other, graphs, want):
+        assert torch.equal(o, w) and torch.equal(c, w)
+
+
+@pytest.mark.gpu
+def test_with_one_map_off_it_is_attention():
+    """lam = 0 leaves the first map: what attention() gives for each half of the values. Both round the same probabilities to fp16."""
+    from fastbb_b200.attention import attention
+    g = torch.Generator("cuda").manual_seed(8)
+    q, k, v, _ = make(1, 390, 390, 2, 2, g)
+    out = diff_attention(q, k, v, torch.zeros((), device="cuda"))
+    for half in (0, 64):
+        one = attention(q[:, :, ::2], k[:, :, ::2], v[..., half:half + 64])
+        assert float((out[..., half:half + 64].float() - one.float()).abs().max()) <= 2.0 ** -9
+
+
+@pytest.mark.gpu
+def test_refusals_on_the_gpu():
+    g = torch.Generator("cuda").manual_seed(7)
+    q, k, v, lam = make(2, 20, 30, 4, 2, g)
+    n = torch.tensor([30, 30], dtype=torch.int32, device="cuda")
+    for call in (
+            lambda: diff_attention(q.float(), k, v, lam), lambda: diff_attention(q, k[..., :32], v, lam), lambda: diff_attention(q, k, v[..., :64], lam),
+            lambda: diff_attention(q[:, :, :7], k, v, lam), lambda: diff_attention(q[:, :, :6], k, v, lam), lambda: diff_attention(q, k, v[:, :29], lam),
+            lambda: diff_attention(q, k[:1], v[:1], lam), lambda: diff_attention(q, k[:1].expand(2, 30, 4, 64), v, lam),
+            lambda: diff_attention(q, k, v, lam.half()), lambda: diff_attention(q, k, v, 0.5), lambda: diff_attention(q, k, v, lam[:3]),
+            lambda: diff_attention(q, k, v, lam.cpu()), lambda: diff_attention(q, k, v, lam, scale=0.0), lambda: diff_attention(q, k, v, lam, scale=float("nan")),
+            lambda: diff_attention(q, k, v, lam, eps=-1.0), lambda: diff_attention(q, k, v, lam, weight=torch.ones(64, device="cuda")),
+            lambda: diff_attention(q, k, v, lam, weight=torch.ones(128, device="cuda").bfloat16()), lambda: diff_attention(q, k, v, lam, key_lengths=n.long()),
+            lambda: diff_attention(q, k, v, lam, key_lengths=n[:1]), lambda: diff_attention(q, k, v, lam, out=torch.empty(2, 20, 4, 64, device="cuda").half()),
+            lambda: diff_attention(q, k, v, lam, out=q.view(2, 20, 4, 128)),
+            lambda: diff_attention(q, k, v, lam, out=torch.empty(1, 20, 4, 128, device="cuda").half().expand(2, 20, 4, 128)),
+            lambda: diff_attention(torch.empty(2, 20, 8, 65, device="cuda").half()[..., 1:], k, v, lam)):
+        with pytest.raises(ValueError):
+            call()
+
+
+# ------------------------------------------------------------------------------------------------------------------ CPU
+def test_cpu_tensors_are_refused():
+    q = torch.zeros(1, 4, 2, 64).half()
+    with pytest.raises(ValueError, match="no fallback"):
+        diff_attention(q, q, torch.zeros(1, 4, 1, 128).half(), torch.zeros(()))
+
+
+def test_entry_point_refusals():
+    lib, A = _lib.load(), 0x7F0000000000
+
+    def call(q=A, k=A, v=A, o=A, B=2, Nq=4, Nk=6, H=4, Hk=2, st=None, lam=A, weight=A, wd=0, eps=1e-5, scale=0.125, ws=None):
+        st = st or [2048, 512, 64, 2048, 256, 64, 2048, 256, 128, 2048, 512, 128]
+        return lib.fbb_diff64_f16(q, k, v, o, B, Nq, Nk, H, Hk, *st, lam, 0, 0, 1, weight, wd, eps, 1.0, scale, None, ws, 0, None)
+
+    assert call(q=None) == call(o=None) == call(lam=None) == call(k=None) == call(v=None) == -1
+    assert call(B=-1) == call(H=0) == call(Hk=3) == call(Hk=0) == call(scale=0.0) == call(scale=float("nan")) == call(eps=-1.0) == -2
+    assert call(q=A + 8) == call(o=A + 2) == call(ws=A + 4) == -3
+    for i in range(12):
+        for value in (0, 12, -64):
+            st = [2048, 512, 64, 2048, 256, 64, 2048, 256, 128, 2048, 512, 128]
+            st[i] = value
+            assert call(st=st) == -3, (i, value)
+    assert call(wd=1) == call(wd=7) == -4
+    assert call(B=0, q=None) == call(Nq=0, o=None) == 0
+    assert lib.fbb_diff64_workspace_bytes(0, 1, 1000, 8) == 0 and lib.fbb_diff64_launches(1, 0, 10, 2) == 0
