@@ -72,6 +72,8 @@ PROTOTYPES = {
     "fbb_flash64_launches": (_i32, [_i32, _i32, _i32, _i32]),
     "fbb_flash64_f16_ws": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _i32] + [_i64] * 12 + [_f32, _i32, _vp, _i64, _vp]),
     "fbb_flash64_f16_static": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _i32] + [_i64] * 12 + [_f32, _i32, _vp]),
+    "fbb_adapter_linear_workspace_bytes": (_i64, [_i64] + [_i32] * 5),
+    "fbb_adapter_linear_f16": (_i32, [_vp] * 6 + [_i64, _i32, _i32] + [_i64] * 4 + [_i32, _vp, _vp, _vp, _i32, _i32, _vp, _vp, _i32, _vp, _i64, _vp]),
     "fbb_diff64_workspace_bytes": (_i64, [_i32] * 4),
     "fbb_diff64_launches": (_i32, [_i32] * 4),
     "fbb_diff64_f16": (_i32, [_vp] * 4 + [_i32] * 5 + [_i64] * 12 + [_vp] + [_i64] * 3 + [_vp, _i32, _f32, _f32, _f32, _vp, _vp, _i64, _vp]),

@@ -278,6 +278,39 @@ int fbb_linear_layernorm_f16(const void* A, const void* W, void* C, const void* 
                                    counter, (cudaStream_t)stream);
 }
 
+int64_t fbb_adapter_linear_workspace_bytes(int64_t M, int N, int K, int epilogue, int rank, int requests) {
+    return adapter_linear_workspace_bytes(M, N, K, epilogue, rank, requests);
+}
+
+int fbb_adapter_linear_f16(const void* A, const void* W, void* C, const void* bias, const void* res, const void* gamma, int64_t M, int N, int K,
+                           int64_t lda, int64_t ldw, int64_t ldc, int64_t ldr, int epilogue, const void* down, const void* up, const float* scale,
+                           int adapters, int rank, const int* ids, const int* offsets, int requests, void* workspace, int64_t workspace_bytes, void* stream) {
+    if (epilogue < FBB_EPI_NONE || epilogue > FBB_EPI_SWIGLU) return fail(FBB_ERR_ENUM, "adapter_linear: unknown epilogue %d", epilogue);
+    if (M < 0 || M > 0x7FFFFF00ll || N <= 0 || K <= 0) return fail(FBB_ERR_SHAPE, "adapter_linear: bad M/N/K (%lld, %d, %d)", (long long)M, N, K);
+    if ((K & 7) != 0 || (N & 7) != 0) return fail(FBB_ERR_SHAPE, "adapter_linear: need K %% 8 == 0 and N %% 8 == 0 (N=%d K=%d)", N, K);
+    const bool swiglu = epilogue == FBB_EPI_SWIGLU;
+    if (swiglu && ((N & 15) != 0 || res != nullptr || gamma != nullptr))
+        return fail(FBB_ERR_SHAPE, "adapter_linear: SwiGLU needs N %% 16 == 0 and no res / gamma");
+    const int n_out = swiglu ? N / 2 : N;
+    if (lda < K || ldw < K || ldc < n_out || (res != nullptr && ldr < n_out))
+        return fail(FBB_ERR_SHAPE, "adapter_linear: a leading dimension is smaller than its row length");
+    if (rank < 8 || rank > 128 || (rank & 7) != 0) return fail(FBB_ERR_SHAPE, "adapter_linear: rank must be a multiple of 8 from 8 to 128, got %d", rank);
+    if (adapters < 1 || (int64_t)adapters * N > 0x7FFFFFFFll) return fail(FBB_ERR_SHAPE, "adapter_linear: need 1 <= adapters and adapters * N < 2^31 (%d, %d)", adapters, N);
+    if (requests < 1 || (offsets == nullptr && M % requests != 0))
+        return fail(FBB_ERR_SHAPE, "adapter_linear: need at least one request, and without offsets the same number of rows for each (%d for %lld rows)", requests, (long long)M);
+    if (M == 0) return FBB_OK;
+    if (A == nullptr || W == nullptr || C == nullptr || down == nullptr || up == nullptr || scale == nullptr || ids == nullptr)
+        return fail(FBB_ERR_NULL, "adapter_linear: A, W, C, down, up, scale or ids is null");
+    if ((lda & 7) || (ldw & 7) || (ldc & 7) || (res != nullptr && (ldr & 7)) || !aligned16(A) || !aligned16(W) || !aligned16(C) || !aligned16(res) ||
+        !aligned16(down) || !aligned16(up) || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)
+        return fail(FBB_ERR_ALIGN, "adapter_linear: A, W, C, res, down, up must be 16-byte aligned (workspace: 256) with leading dimensions %% 8 == 0");
+    const uintptr_t a0 = reinterpret_cast<uintptr_t>(A), c0 = reinterpret_cast<uintptr_t>(C);
+    if (a0 < c0 + 2 * (uintptr_t)((M - 1) * ldc + n_out) && c0 < a0 + 2 * (uintptr_t)((M - 1) * lda + K))
+        return fail(FBB_ERR_SHAPE, "adapter_linear: C shares memory with A");
+    return launch_adapter_linear(A, W, C, bias, res, gamma, M, N, K, lda, ldw, ldc, ldr, epilogue, down, up, scale, adapters, rank, ids, offsets, requests,
+                                 workspace, workspace_bytes, (cudaStream_t)stream);
+}
+
 int64_t fbb_diff64_workspace_bytes(int B, int Nq, int Nk, int H) { return diff64_workspace_bytes(B, Nq, Nk, H); }
 int fbb_diff64_launches(int B, int Nq, int Nk, int H) { return diff64_launches(B, Nq, Nk, H); }
 

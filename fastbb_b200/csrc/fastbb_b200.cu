@@ -2,6 +2,7 @@
 // helpers, so they are compiled together (no relocatable device code, no device link step).
 #include "layernorm.cu"
 #include "gemm.cu"
+#include "adapters.cu"
 #include "flash64.cu"
 #include "diff64.cu"
 #include "rotary.cu"

@@ -122,10 +122,21 @@ __device__ __forceinline__ void remainder_rows_by_gemv(const GemmArgs& g, bool s
     }
 }
 
-template <int BN, bool SWIGLU, bool CTA2, bool SLICES = false>
-__global__ void __launch_bounds__(kGemmThreads, 1)
-linear_umma_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w,
-                   const __grid_constant__ CUtensorMap tmap_wn, const __grid_constant__ CUtensorMap tmap_c, const GemmArgs g) {
+// What a launch beside the shared projection adds (adapters.cu): of every row tile the products of its requests' adapters.
+enum AdaptMode { kAdaptNone, kAdaptBlocks, kAdaptRows };
+struct AdaptArgs {
+    const int4* tiles;         // blocks: of each row tile {first request, one behind its last, products to add, 0}
+    const int* list;           // blocks: adapter of request s in tile t at t + s, -1: none; rows: of each row
+    const __half* h;           // rows: [M, r], what the adapters' first matrices made of the rows of A, times their scale
+    const __half* up;          // rows: the second matrices [adapters, N, r]
+    const CUtensorMap* map_h;  // blocks: the same per tile and request, [(t + s) * tile rows, r], rows of other requests zero
+    const CUtensorMap* map_up;
+    int r, r_blocks;           // rank, and the 64-element k-blocks it takes
+};
+
+template <int BN, bool SWIGLU, bool CTA2, bool SLICES, AdaptMode ADAPT>
+__device__ __forceinline__ void linear_umma_body(const CUtensorMap& tmap_a, const CUtensorMap& tmap_w, const CUtensorMap& tmap_wn, const CUtensorMap& tmap_c,
+                                                 const GemmArgs& g, const AdaptArgs& ad) {
     using S = GemmSmem<BN, CTA2>;
     // pair geometry: rank 0 (the leader) issues the UMMAs; work items are 256-row tiles shared by the pair
     const uint32_t rank = CTA2 ? cluster_ctarank() : 0u;
@@ -198,7 +209,9 @@ linear_umma_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
     if constexpr (CTA2) cluster_sync_all();  // both CTAs' barriers exist before either signals the other
     tc_fence_after();
     const uint32_t tmem_base = *s_tmem;
-    grid_dependency_wait();  // the set-up above may overlap the previous kernel's tail; its outputs are visible from here
+    // The set-up above may overlap the previous kernel's tail; its outputs are visible from here. A launch with adapters runs behind
+    // the kernel that makes h, which depends on everything this one reads but h, so only what reads h (and its tables) waits for it.
+    if constexpr (ADAPT == kAdaptNone) grid_dependency_wait();
     grid_launch_dependents();
 
     if (warp == 0) {
@@ -231,6 +244,32 @@ linear_umma_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
                     }
                     if (++s == kStages) { s = 0; ph ^= 1u; }
                 }
+                if constexpr (ADAPT == kAdaptBlocks) {
+                    // the adapters of the tile's requests: k-blocks of h (zero outside the request's rows) and of the adapter's second matrix
+                    grid_dependency_wait();
+                    const int tile = item / g.tiles_n;
+                    const int4 of = __ldcg(ad.tiles + tile);
+                    for (int s0 = of.x; s0 < of.y && ok; s0 += 32) {
+                        const int slot = s0 + lane < of.y ? __ldcg(ad.list + tile + s0 + lane) : -1;
+                        for (uint32_t todo = __ballot_sync(0xffffffffu, slot >= 0); todo != 0u && ok; todo &= todo - 1u) {
+                            const int i = __ffs(todo) - 1;
+                            const int up0 = __shfl_sync(0xffffffffu, slot, i) * g.N, h0 = (tile + s0 + i) * kTileRows + (int)rank * BM;
+                            for (int kb = 0; kb < ad.r_blocks; ++kb) {
+                                if (__all_sync(0xffffffffu, mbar_wait(empty_bar(s), ph ^ 1u, s_abort, DEV_TIMEOUT_SMEM_EMPTY, s)) == 0) { ok = false; break; }
+                                const uint32_t sa = base + s * S::kStageBytes;
+                                const uint32_t sb = sa + S::kABytes;
+                                if constexpr (CTA2) {
+                                    const int wrow = SWIGLU ? (rank == 0 ? nt * (BN / 2) : g.N / 2 + nt * (BN / 2)) : nt * BN + (int)rank * (BN / 2);
+                                    tma_load_2d_two_pair_warp(full_bar(s), rank == 0 ? 2u * S::kStageBytes : 0u, sa, ad.map_h, kb * BK, h0, sb, ad.map_up, kb * BK, up0 + wrow);
+                                } else {
+                                    tma_load_2d_two_warp(full_bar(s), S::kStageBytes, sa, ad.map_h, kb * BK, h0, sb, ad.map_up, kb * BK, up0 + (SWIGLU ? nt * (BN / 2) : nt * BN));
+                                    if (SWIGLU) tma_load_2d_warp(sb + S::kBBytes / 2, ad.map_up, full_bar(s), kb * BK, up0 + g.N / 2 + nt * (BN / 2));
+                                }
+                                if (++s == kStages) { s = 0; ph ^= 1u; }
+                            }
+                        }
+                    }
+                }
             }
             if (!ok) __nanosleep(20000);  // let copies already in flight land before the CTA leaves
         }
@@ -253,7 +292,8 @@ linear_umma_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
             if (!all_ok(mbar_wait(tempty_bar(acc), acc_ph ^ 1u, s_abort, DEV_TIMEOUT_TMEM_EMPTY, acc))) break;
             tc_fence_after();
             const uint32_t d_tmem = tmem_base + (uint32_t)(acc * BN);
-            for (int kb = 0; kb < num_kb; ++kb) {
+            int total_kb = num_kb;
+            for (int kb = 0; kb < total_kb; ++kb) {
                 if (!all_ok(mbar_wait(full_bar(s), ph, s_abort, DEV_TIMEOUT_TMA_FULL, s))) { ok = false; break; }
                 tc_fence_after();
                 const uint64_t adesc = adesc0 + (uint64_t)(s * (S::kStageBytes >> 4));
@@ -264,6 +304,12 @@ linear_umma_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
                     umma_kblock_commit_warp(d_tmem, adesc, bdesc, idesc, kb != 0 ? 1u : 0u, empty_bar(s));  // stage reusable once these UMMAs have read it
                 }
                 if (++s == kStages) { s = 0; ph ^= 1u; }
+                if constexpr (ADAPT == kAdaptBlocks) {
+                    if (kb + 1 == num_kb) {
+                        grid_dependency_wait();
+                        total_kb = num_kb + __ldcg(ad.tiles + item / g.tiles_n).z * ad.r_blocks;
+                    }
+                }
             }
             if (!ok) break;
             if constexpr (CTA2) umma_commit_pair_warp(tfull_bar(acc));  // both CTAs' accumulators complete
@@ -317,6 +363,35 @@ linear_umma_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
                     }
                 }
             }
+            // This thread's row of h times the rows of its adapter's second matrix that belong to columns n .. n + 31, on the CUDA cores:
+            // where requests have few rows, a k-block per request and tile costs more.
+            int slot = -1;
+            if constexpr (ADAPT == kAdaptRows) {
+                grid_dependency_wait();
+                if (row_ok) slot = __ldcg(ad.list + row);
+            }
+            auto add_adapter = [&](float* v, int n) {
+                if (slot < 0) return;
+                const uint4* hr = reinterpret_cast<const uint4*>(ad.h + (int64_t)row * ad.r);
+                const uint4* up = reinterpret_cast<const uint4*>(ad.up + (int64_t)slot * g.N * ad.r);
+                const int vecs = ad.r >> 3;  // a row's 16-byte vectors
+                for (int p = 0; p < vecs; ++p) {
+                    const uint4 hv = __ldcg(hr + p);
+                    const __half2* hh = reinterpret_cast<const __half2*>(&hv);
+                    float2 hf[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) hf[e] = __half22float2(hh[e]);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        const uint4 uv = __ldg(up + (int64_t)min(n + j, g.N - 1) * vecs + p);  // (a column beyond the last is not stored)
+                        const __half2* uh = reinterpret_cast<const __half2*>(&uv);
+                        float2 sum = make_float2(v[j], 0.f);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) sum = ffma2(hf[e], __half22float2(uh[e]), sum);
+                        v[j] = sum.x + sum.y;
+                    }
+                }
+            };
             if (!mbar_wait(tfull_bar(acc), acc_ph, s_abort, DEV_TIMEOUT_TMEM_FULL, acc)) break;
             tc_fence_after();
             const uint32_t t_row = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * BN);
@@ -335,10 +410,19 @@ linear_umma_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
 #pragma unroll
                     for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
                 }
+                if constexpr (ADAPT == kAdaptRows) add_adapter(v, n0 + c0);
                 if (SWIGLU) {
                     uint32_t r2[32];
                     tmem_ld32(t_row + (uint32_t)(BN / 2 + c0), r2);
                     tmem_wait_ld();
+                    if constexpr (ADAPT == kAdaptRows) {
+                        float v2[32];
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v2[j] = __uint_as_float(r2[j]);
+                        add_adapter(v2, g.N / 2 + n0 + c0);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) r2[j] = __float_as_uint(v2[j]);
+                    }
 #pragma unroll
                     for (int j = 0; j < 32; ++j) {
                         const float x2 = (g.acc_f16 ? __half2float(__ushort_as_half((unsigned short)(r2[j] & 0xFFFFu)))
@@ -404,6 +488,7 @@ linear_umma_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
         if (lane == 0) bulk_wait_all();  // this warp's output stores are complete before the CTA gives up its shared memory
     }
 
+    if constexpr (ADAPT != kAdaptNone) grid_dependency_wait();  // whoever waits for this grid finds the kernel ahead of it complete as well
     tc_fence_before();
     __syncthreads();
     if constexpr (CTA2) cluster_sync_all();  // the peer may still be signalling this CTA's barriers / reading its operands
@@ -413,6 +498,13 @@ linear_umma_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_cons
         if constexpr (CTA2) tmem_dealloc_pair<2 * BN>(tmem_base);
         else tmem_dealloc<2 * BN>(tmem_base);
     }
+}
+
+template <int BN, bool SWIGLU, bool CTA2, bool SLICES = false>
+__global__ void __launch_bounds__(kGemmThreads, 1)
+linear_umma_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w,
+                   const __grid_constant__ CUtensorMap tmap_wn, const __grid_constant__ CUtensorMap tmap_c, const GemmArgs g) {
+    linear_umma_body<BN, SWIGLU, CTA2, SLICES, kAdaptNone>(tmap_a, tmap_w, tmap_wn, tmap_c, g, AdaptArgs{});
 }
 
 // ---------------------------------------------------------------------------------------------------------------------

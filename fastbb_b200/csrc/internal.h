@@ -102,6 +102,12 @@ int flash64_static_workspace(void** ptr, int64_t* bytes, cudaStream_t stream);
 int64_t flash64_workspace_bytes_for(int B, int N, int H);
 int flash64_launches(int B, int N, int H, bool has_workspace);
 
+// A linear layer with the low-rank adapters of many requests (adapters.cu).
+int64_t adapter_linear_workspace_bytes(int64_t M, int N, int K, int epilogue, int r, int S);
+int launch_adapter_linear(const void* A, const void* W, void* C, const void* bias, const void* res, const void* gamma, int64_t M, int N, int K, int64_t lda,
+                          int64_t ldw, int64_t ldc, int64_t ldr, int epilogue, const void* down, const void* up, const float* scale, int L, int r, const int* ids,
+                          const int* offsets, int S, void* ws, int64_t ws_bytes, cudaStream_t stream);
+
 // Differential attention (diff64.cu). Strides in elements, {batch, token, head} each; ls: lam's.
 int64_t diff64_workspace_bytes(int B, int Nq, int Nk, int H);
 int diff64_launches(int B, int Nq, int Nk, int H);

@@ -192,6 +192,23 @@ int fbb_flash64_f16_static(const void* q, const void* k, const void* v, void* o,
                            int64_t q_sh, int64_t k_sb, int64_t k_sn, int64_t k_sh, int64_t v_sb, int64_t v_sn, int64_t v_sh,
                            int64_t o_sb, int64_t o_sn, int64_t o_sh, float scale, int variant, void* stream);
 
+/* ---- a linear layer with the low-rank adapters of many requests ---------------------------------------------------------------
+ * C = epilogue(A . W^T + scale_a (A . down_a^T) . up_a^T), a the adapter of the row's request: one shared projection for fine-tuned variants
+ * of a model served together. The layer itself is fbb_linear_f16's (same arguments, epilogues and requirements; fp32 accumulator); C may
+ * share memory with res (same pointer and stride) but not with A. No counterpart in the reference.
+ * down: [adapters, rank, K], up: [adapters, N, rank], fp16, contiguous, 16-byte aligned; scale: [adapters] fp32. rank: a multiple of 8 up to
+ * 128 (smaller ones are padded with zeros by the caller). ids: int32 [requests], an id out of [0, adapters) means no adapter.
+ * offsets: int32 [requests + 1], not decreasing: request s has rows offsets[s] .. offsets[s + 1] - 1; rows of no request have no adapter. null:
+ * M / requests rows each (a whole number). Both are read on the device; offsets that decrease give wrong results for the rows they
+ * concern, nothing else. adapters * N < 2^31.
+ * A . down_a^T times scale is rounded to fp16 ahead of the second product; everything else is fp32.
+ * workspace: fbb_adapter_linear_workspace_bytes() of 256-byte aligned device memory, overwritten freely; calls that may overlap in time need
+ * different ones. Two kernels are enqueued. */
+int64_t fbb_adapter_linear_workspace_bytes(int64_t M, int N, int K, int epilogue, int rank, int requests);
+int fbb_adapter_linear_f16(const void* A, const void* W, void* C, const void* bias, const void* res, const void* gamma, int64_t M, int N, int K,
+                           int64_t lda, int64_t ldw, int64_t ldc, int64_t ldr, int epilogue, const void* down, const void* up, const float* scale,
+                           int adapters, int rank, const int* ids, const int* offsets, int requests, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* ---- differential attention -----------------------------------------------------------------------------------------------
  * o = softmax(scale q1 k1^T) v - lam softmax(scale q2 k2^T) v: two maps of head dimension 64 over the same values of 128 columns;
  * with a weight followed by the norm of every row of 128, o * weight / sqrt(mean(o^2) + eps); both times out_scale. No counterpart
