@@ -1,14 +1,14 @@
 // One shared projection and the low-rank adapters of many requests beside it: rows [offsets[s], offsets[s + 1]) belong to request s, whose
 // adapter a = ids[s] adds scale_a (x A_a^T) B_a^T to x W^T ahead of the bias and the activation (A_a [r, K], B_a [N, r]).
 //
-// Two launches: one makes h = scale (x A_a^T), rounded to fp16 because the tensor cores take it so (2^-11 of each value, as the
+// Two launches: one makes h = scale (x A_a^T), rounded (in the blocks form) to fp16 because the tensor cores take it so (2^-11 of each value, as the
 // projection's own output is rounded), and the linear kernel adds h B_a^T to the accumulator it holds anyway. The second launch starts
 // under the first (its product with W needs nothing of it) and waits for it where it needs h. Two forms of the pair:
 //  blocks  h is laid out per (row tile t, request s in it) as block t + s of a tile's rows with zeros outside the request's (the
 //          requests of one tile follow one another, so t + s is a number of its own), and the linear kernel runs each as k-blocks behind
 //          those of x and W: one k-block of 64 per request and tile for ranks up to 64.
-//  rows    for requests of few rows, where that would be a k-block per row or so: h is [M, r], and the epilogue multiplies each
-//          row with its adapter's rows of B on the CUDA cores.
+//  rows    for few rows of many requests, where that would be a k-block per row or so: the first launch multiplies each row with both
+//          of its adapter's matrices on the CUDA cores (bound by reading those), and the linear kernel's epilogue adds that in fp32.
 // Rows of no request (ahead of offsets[0], behind offsets[S]) and of requests with an id out of [0, adapters) get x W^T alone.
 #include "common.cuh"
 #include "internal.h"
@@ -22,11 +22,16 @@ struct AdapterArgs {
     const float* scale;   // [L]
     const int* ids;       // [S]
     const int* offsets;   // [S + 1] or null: `each` rows a request
-    int M, K, L, r, S, each;
-    int tile_rows;        // blocks form
+    int M, N, K, L, r, S, each;
+    // blocks form
+    int tile_rows;
     __half* h;
     int4* tiles;
     int* list;
+    // rows form
+    const __half* up;     // [L, N, r]
+    float* delta;
+    int cols;
 };
 
 __device__ __forceinline__ int adapter_begin(const AdapterArgs& a, int s) {
@@ -52,100 +57,221 @@ __device__ __forceinline__ int adapter_request(const AdapterArgs& a, int row, in
     return lo;
 }
 
-__device__ __forceinline__ void mma_m16n8k16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
+// h of the blocks form: a CTA takes 128 rows of x and multiplies them with the first matrices of their requests, up to 64 columns of
+// h at a time (several requests side by side where the rank leaves room), as UMMAs of 128 x 64 fed by TMA: x is read once for most tiles,
+// and the launch is bound by that. x's tiles start ahead of the look-up of the requests, which is a chain of dependent loads. The
+// first CTA of a row tile also writes the tables that the linear kernel goes by.
+//   warp 0   look-up of the requests, then TMA producer      warp 1   UMMA issuer      warps 2..5   rows of h out of tensor memory
+constexpr int kDownCols = 64;     // of h in a pass
+constexpr int kDownStages = 4;
+constexpr int kDownMaxRequests = 128;
+constexpr int kDownThreads = 192;
+struct DownSmem {
+    static constexpr int kABytes = BM * BK * 2;
+    static constexpr int kStageBytes = kABytes + kDownCols * BK * 2;
+    static constexpr int kBarOff = kDownStages * kStageBytes;
+    static constexpr int kNumBars = 2 * kDownStages + 4;  // full, empty, accumulator full[2], empty[2]
+    static constexpr int kTableOff = kBarOff + kNumBars * 8 + 16;
+    static constexpr int kDynamic = 1024 + kTableOff + (int)(kDownMaxRequests * sizeof(int4)) + 16;
+};
 
-// h of the blocks form. A CTA takes 32 rows of x and, of every request among them, all r products: 4 warps share K, 16-byte loads
-// straight into fragments (the order of K inside a fragment is free as long as both operands agree), partial sums joined in shared
-// memory in a fixed order. The launch reads x once (bound by that and by latency): mma.sync with its operands in registers is the
-// shortest way for products of 32 x r. The first CTA of a tile also writes the tables that the linear kernel goes by.
-constexpr int kDownRows = 32, kDownWarps = 4;
-template <int NT>  // r in chunks of 8 NT
-__global__ void __launch_bounds__(kDownWarps * 32) adapter_down_blocks_kernel(const AdapterArgs a) {
-    __shared__ float s_part[kDownWarps][kDownRows][8 * NT + 1];
+__global__ void __launch_bounds__(kDownThreads) adapter_down_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_down,
+                                                                    const AdapterArgs a) {
+    using S = DownSmem;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+    uint8_t* gen = smem_raw + (base - raw);
+    const uint32_t bar0 = base + S::kBarOff;
+    auto full_bar = [&](int s) { return bar0 + 8u * s; };
+    auto empty_bar = [&](int s) { return bar0 + 8u * (kDownStages + s); };
+    auto tfull_bar = [&](int i) { return bar0 + 8u * (2 * kDownStages + i); };
+    auto tempty_bar = [&](int i) { return bar0 + 8u * (2 * kDownStages + 2 + i); };
+    volatile uint32_t* s_tmem = reinterpret_cast<volatile uint32_t*>(gen + S::kBarOff + S::kNumBars * 8);
+    volatile int* s_abort = reinterpret_cast<volatile int*>(gen + S::kBarOff + S::kNumBars * 8 + 4);
+    int4* s_req = reinterpret_cast<int4*>(gen + S::kTableOff);  // {request, first row, one behind its last, adapter}
+    volatile int* s_count = reinterpret_cast<volatile int*>(s_req + kDownMaxRequests);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int num_kb = (a.K + BK - 1) / BK;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kDownStages; ++s) {
+            mbar_init(full_bar(s), 2);  // x's bytes, the adapters' bytes
+            mbar_init(empty_bar(s), 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(tfull_bar(i), 1);
+            mbar_init(tempty_bar(i), 4);
+        }
+        *s_abort = 0;
+        fence_barrier_init();
+        tma_prefetch_desc(&tmap_x);
+        tma_prefetch_desc(&tmap_down);
+    }
+    if (warp == 1) {
+        __syncwarp();
+        tmem_alloc<2 * kDownCols>(smem_u32(const_cast<uint32_t*>(s_tmem)));
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *s_tmem;
     grid_dependency_wait();
     grid_launch_dependents();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int m0 = (int)blockIdx.x * kDownRows, m1 = min(m0 + kDownRows, a.M);
+
+    const int m0 = (int)blockIdx.x * BM, m1 = min(m0 + BM, a.M);
     const int tile = m0 / a.tile_rows, t0 = tile * a.tile_rows, t1 = min(t0 + a.tile_rows, a.M);
-    const int first = adapter_request(a, t0, lane), end = min(adapter_request(a, t1 - 1, lane) + 1, a.S);
-    if (m0 == t0 && warp == 0) {
-        int count = 0;
+    const int ahead = min(num_kb, kDownStages);
+    if (warp == 0) {
+        if (lane == 0) {
+            for (int s = 0; s < ahead; ++s) {
+                mbar_arrive_expect_tx(full_bar(s), S::kABytes);
+                tma_load_2d(base + s * S::kStageBytes, &tmap_x, full_bar(s), s * BK, m0);
+            }
+        }
+        __syncwarp();
+        const int first = adapter_request(a, t0, lane), end = min(adapter_request(a, t1 - 1, lane) + 1, a.S);
+        int count = 0, here = 0;
         for (int s0 = first; s0 < end; s0 += 32) {
             const int s = s0 + lane;
-            int id = -1;
-            if (s < end && max(adapter_begin(a, s), t0) < min(adapter_begin(a, s + 1), t1)) id = adapter_id(a, s);
-            if (s < end) a.list[tile + s] = id;
-            count += __popc(__ballot_sync(0xffffffffu, id >= 0));
+            int id = -1, b = 0, e = 0;
+            if (s < end) {
+                b = adapter_begin(a, s);
+                e = adapter_begin(a, s + 1);
+                if (max(b, t0) < min(e, t1)) id = adapter_id(a, s);
+                if (m0 == t0) a.list[tile + s] = id;
+            }
+            const uint32_t any = __ballot_sync(0xffffffffu, id >= 0), mine = __ballot_sync(0xffffffffu, id >= 0 && max(b, m0) < min(e, m1));
+            const int at = here + __popc(mine & ((1u << lane) - 1u));
+            if (((mine >> lane) & 1u) != 0u && at < kDownMaxRequests) s_req[at] = make_int4(s, b, e, id);
+            // of the tile's requests, those with no rows among this CTA's leave zeros here
+            for (uint32_t rest = any & ~mine; rest != 0u; rest &= rest - 1u) {
+                uint4* dst = reinterpret_cast<uint4*>(a.h + ((int64_t)(tile + s0 + __ffs(rest) - 1) * a.tile_rows + (m0 - t0)) * a.r);
+                for (int i = lane; i < BM * (a.r >> 3); i += 32) dst[i] = make_uint4(0u, 0u, 0u, 0u);
+            }
+            count += __popc(any);
+            here += __popc(mine);
         }
-        if (lane == 0) a.tiles[tile] = make_int4(first, end, count, 0);
+        if (lane == 0) {
+            *s_count = min(here, kDownMaxRequests);
+            if (m0 == t0) a.tiles[tile] = make_int4(first, end, count, 0);
+        }
     }
-    const int g = lane >> 2, q = lane & 3;
-    for (int s = first; s < end; ++s) {
-        const int b = adapter_begin(a, s), e = adapter_begin(a, s + 1), id = adapter_id(a, s);
-        if (id < 0 || max(b, t0) >= min(e, t1)) continue;
-        __half* dst = a.h + ((int64_t)(tile + s) * a.tile_rows + (m0 - t0)) * a.r;
-        if (max(b, m0) >= min(e, m1)) {  // none of its rows are here
-            for (int i = threadIdx.x; i < kDownRows * (a.r >> 3); i += kDownWarps * 32) reinterpret_cast<uint4*>(dst)[i] = make_uint4(0u, 0u, 0u, 0u);
-            continue;
-        }
-        const float scale = __ldcg(a.scale + id);
-        for (int n0 = 0; n0 < a.r; n0 += 8 * NT) {
-            float acc[2][NT][4] = {};
-            const __half* down = a.down + ((int64_t)id * a.r + n0 + g) * a.K;
-            const __half* x[4];  // rows g, g + 8, g + 16, g + 24; beyond the last row the last one again
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = a.x + (int64_t)min(m0 + g + 8 * i, a.M - 1) * a.ldx;
-#pragma unroll 2
-            for (int k = (warp * 4 + q) * 8; k < (a.K + 31) / 32 * 32; k += kDownWarps * 32) {
-                uint4 xv[4], dv[NT];
-                const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) xv[i] = k < a.K ? *reinterpret_cast<const uint4*>(x[i] + k) : zero;
-#pragma unroll
-                for (int n = 0; n < NT; ++n) dv[n] = (k < a.K && n0 + 8 * n < a.r) ? __ldg(reinterpret_cast<const uint4*>(down + (int64_t)(8 * n) * a.K + k)) : zero;
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        mma_m16n8k16(acc[i][n], xv[2 * i].x, xv[2 * i + 1].x, xv[2 * i].y, xv[2 * i + 1].y, dv[n].x, dv[n].y);
-                        mma_m16n8k16(acc[i][n], xv[2 * i].z, xv[2 * i + 1].z, xv[2 * i].w, xv[2 * i + 1].w, dv[n].z, dv[n].w);
+    __syncthreads();
+    // Passes: columns [c0, c0 + cols) of the requests' r columns each, side by side; a rank above 64 takes two passes a request.
+    const int requests = *s_count, per_pass = a.r >= kDownCols ? 1 : kDownCols / a.r;
+    const int halves = a.r > kDownCols ? 2 : 1, passes = (requests + per_pass - 1) / per_pass * halves;
+    auto pass_at = [&](int p, int& req0, int& n, int& c0, int& cols) {
+        req0 = p / halves * per_pass;
+        n = min(per_pass, requests - req0);
+        c0 = (p % halves) * kDownCols;
+        cols = min(kDownCols, a.r - c0);
+    };
+    if (warp == 0) {
+        if (lane == 0) {
+            int s = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            for (int p = 0; p < passes && ok; ++p) {
+                int req0, n, c0, cols;
+                pass_at(p, req0, n, c0, cols);
+                for (int kb = 0; kb < num_kb; ++kb) {
+                    const uint32_t st = base + s * S::kStageBytes;
+                    if (p > 0 || kb >= ahead) {
+                        if (!mbar_wait(empty_bar(s), ph ^ 1u, s_abort, DEV_TIMEOUT_SMEM_EMPTY, s)) { ok = false; break; }
+                        mbar_arrive_expect_tx(full_bar(s), S::kABytes);
+                        tma_load_2d(st, &tmap_x, full_bar(s), kb * BK, m0);
                     }
+                    // boxes of min(64, r) rows, which may reach into the next adapter's: they land behind this request's, or nowhere that is read
+                    mbar_arrive_expect_tx(full_bar(s), (uint32_t)(n * min(kDownCols, a.r) * BK * 2));
+                    for (int i = 0; i < n; ++i)
+                        tma_load_2d(st + S::kABytes + (uint32_t)(i * cols * BK * 2), &tmap_down, full_bar(s), kb * BK, s_req[req0 + i].w * a.r + c0);
+                    if (++s == kDownStages) { s = 0; ph ^= 1u; }
+                }
             }
-            __syncthreads();  // the previous sums have been read
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) s_part[warp][16 * i + g + 8 * (j >> 1)][8 * n + 2 * q + (j & 1)] = acc[i][n][j];
-            __syncthreads();
-            const int cols = min(8 * NT, a.r - n0);
-            for (int i = threadIdx.x; i < kDownRows * (cols >> 1); i += kDownWarps * 32) {
-                const int row = i / (cols >> 1), c = 2 * (i - row * (cols >> 1));
-                float v0 = 0.f, v1 = 0.f;
-#pragma unroll
-                for (int w = 0; w < kDownWarps; ++w) v0 += s_part[w][row][c], v1 += s_part[w][row][c + 1];
-                const bool mine = m0 + row >= b && m0 + row < e;
-                *reinterpret_cast<uint32_t*>(dst + (int64_t)row * a.r + n0 + c) = mine ? pack_h2(v0 * scale, v1 * scale) : 0u;
-            }
+            if (passes == 0)  // nobody waits for what was sent ahead, but it must land before the CTA leaves
+                for (int i = 0; i < ahead; ++i) {
+                    mbar_arrive(full_bar(i));
+                    ok = ok && mbar_wait(full_bar(i), 0, s_abort, DEV_TIMEOUT_TMA_FULL, i);
+                }
+            if (!ok) __nanosleep(20000);
         }
+    } else if (warp == 1) {
+        constexpr uint64_t desc_hi = make_smem_desc_hi(16, 1024);
+        const uint64_t adesc0 = smem_desc(base, desc_hi);
+        auto all_ok = [&](bool mine) { return __all_sync(0xffffffffu, mine) != 0; };
+        int s = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        for (int p = 0; p < passes && ok; ++p) {
+            int req0, n, c0, cols;
+            pass_at(p, req0, n, c0, cols);
+            const int acc = p & 1;
+            ok = all_ok(mbar_wait(tempty_bar(acc), (((uint32_t)p >> 1) & 1u) ^ 1u, s_abort, DEV_TIMEOUT_TMEM_EMPTY, acc));
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t idesc = make_idesc_f16(BM, (n * cols + 15) / 16 * 16, true, false, false);
+            for (int kb = 0; kb < num_kb; ++kb) {
+                if (!all_ok(mbar_wait(full_bar(s), ph, s_abort, DEV_TIMEOUT_TMA_FULL, s))) { ok = false; break; }
+                tc_fence_after();
+                const uint64_t adesc = adesc0 + (uint64_t)(s * (S::kStageBytes >> 4));
+                umma_kblock_commit_warp(tmem_base + (uint32_t)(acc * kDownCols), adesc, adesc + (uint64_t)(S::kABytes >> 4), idesc, kb != 0 ? 1u : 0u, empty_bar(s));
+                if (++s == kDownStages) { s = 0; ph ^= 1u; }
+            }
+            if (ok) umma_commit_warp(tfull_bar(acc));
+        }
+    } else {
+        const int quad = warp & 3, row = m0 + quad * 32 + lane;
+        for (int p = 0; p < passes; ++p) {
+            int req0, n, c0, cols;
+            pass_at(p, req0, n, c0, cols);
+            const int acc = p & 1;
+            if (!mbar_wait(tfull_bar(acc), ((uint32_t)p >> 1) & 1u, s_abort, DEV_TIMEOUT_TMEM_FULL, acc)) break;
+            tc_fence_after();
+            for (int i = 0; i < n; ++i) {
+                const int4 req = s_req[req0 + i];
+                const float scale = row >= req.y && row < req.z ? __ldcg(a.scale + req.w) : 0.f;
+                const bool mine = row >= req.y && row < req.z;
+                uint4* dst = reinterpret_cast<uint4*>(a.h + ((int64_t)(tile + req.x) * a.tile_rows + (row - t0)) * a.r + c0);
+                for (int c = 0; c < cols; c += 8) {
+                    uint32_t v[8];
+                    tmem_ld8(tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * kDownCols + i * cols + c), v);
+                    tmem_wait_ld();
+                    // rows of other requests are zeros, whatever their products are
+                    dst[c >> 3] = mine ? make_uint4(pack_h2(__uint_as_float(v[0]) * scale, __uint_as_float(v[1]) * scale), pack_h2(__uint_as_float(v[2]) * scale, __uint_as_float(v[3]) * scale),
+                                                    pack_h2(__uint_as_float(v[4]) * scale, __uint_as_float(v[5]) * scale), pack_h2(__uint_as_float(v[6]) * scale, __uint_as_float(v[7]) * scale))
+                                       : make_uint4(0u, 0u, 0u, 0u);
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(tempty_bar(acc));
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        __syncwarp();
+        tc_fence_after();
+        tmem_dealloc<2 * kDownCols>(tmem_base);
     }
 }
 
-// h of the rows form: one CTA per row, its warps take the r products in turn.
-__global__ void __launch_bounds__(256) adapter_down_rows_kernel(const AdapterArgs a) {
+// The rows form's adapters: delta[m, n] = scale (x[m] A_a^T) B_a^T in fp32, which the linear kernel's epilogue adds. One CTA per row and
+// `cols` of its columns (a few CTAs share a row where there are few rows): the r products in turn by its warps, then a column per thread.
+__global__ void __launch_bounds__(256) adapter_rows_kernel(const AdapterArgs a) {
+    __shared__ __align__(16) float s_h[128];
     grid_dependency_wait();
     grid_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int m = (int)blockIdx.x;
+    const int m = (int)blockIdx.x, n0 = (int)blockIdx.y * a.cols, n1 = min(n0 + a.cols, a.N);
     const int s = adapter_request(a, m, lane);
     const int id = s < a.S && adapter_begin(a, s) <= m ? adapter_id(a, s) : -1;
-    if (threadIdx.x == 0) a.list[m] = id;
-    if (id < 0) return;
+    float* delta = a.delta + (int64_t)m * a.N;
+    if (id < 0) {
+        for (int n = n0 + threadIdx.x; n < n1; n += 256) delta[n] = 0.f;
+        return;
+    }
     const uint4* x = reinterpret_cast<const uint4*>(a.x + (int64_t)m * a.ldx);
     const int vecs = a.K >> 3;
     const float scale = __ldcg(a.scale + id);
@@ -162,7 +288,20 @@ __global__ void __launch_bounds__(256) adapter_down_rows_kernel(const AdapterArg
         float sum = acc.x + acc.y;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (lane == 0) a.h[(int64_t)m * a.r + n] = __float2half_rn(sum * scale);
+        if (lane == 0) s_h[n] = sum * scale;
+    }
+    __syncthreads();
+    for (int n = n0 + threadIdx.x; n < n1; n += 256) {
+        const uint4* u = reinterpret_cast<const uint4*>(a.up + ((int64_t)id * a.N + n) * a.r);
+        float2 acc = make_float2(0.f, 0.f);
+#pragma unroll 2
+        for (int v = 0; v < (a.r >> 3); ++v) {
+            const uint4 uv = __ldg(u + v);
+            const __half2* uh = reinterpret_cast<const __half2*>(&uv);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc = ffma2(*reinterpret_cast<const float2*>(s_h + 8 * v + 2 * e), __half22float2(uh[e]), acc);
+        }
+        delta[n] = acc.x + acc.y;
     }
 }
 
@@ -185,11 +324,10 @@ static AdapterForm adapter_form(int64_t M, int N, int K, bool swiglu, int r, int
     const int n_out = swiglu ? N / 2 : N, sms = num_sms();
     AdapterForm f = {};
     auto tiles = [&](int rows, int bn) { return ((M + rows - 1) / rows) * (int64_t)((n_out + (swiglu ? bn / 2 : bn) - 1) / (swiglu ? bn / 2 : bn)); };
-    f.rows = M < 8 * (int64_t)S;
+    f.rows = M < 8 * (int64_t)S && M <= 512;
+    if (const char* e = getenv("FBB_ADAPTER_FORM")) f.rows = e[0] == 'r';  // rows | blocks: tuning and test aid
     const int pairs = gemm_pairs_enabled() ? (swiglu ? max_pairs<256, true>() : max_pairs<256, false>()) : 0;
-    if (f.rows) {
-        f.bn = !swiglu && tiles(BM, 128) <= sms / 2 ? 64 : 128;
-    } else if (pairs > 0 && tiles(2 * BM, 256) > pairs / 2) {
+    if (!f.rows && pairs > 0 && tiles(2 * BM, 256) > pairs / 2) {
         f.bn = 256;
         f.pairs = true;
     } else {
@@ -198,23 +336,27 @@ static AdapterForm adapter_form(int64_t M, int N, int K, bool swiglu, int r, int
     return f;
 }
 
-// Workspace: h, then the tile table, then the list, each on a 256-byte boundary.
+// Workspace: h, the tile table and the list of the blocks form, each on a 256-byte boundary, or the rows form's delta.
 struct AdapterSpace {
     int64_t tiles, list, bytes;
 };
-static AdapterSpace adapter_space(const AdapterForm& f, int64_t M, int r, int S) {
-    AdapterSpace w;
+static AdapterSpace adapter_space(const AdapterForm& f, int64_t M, int N, int r, int S) {
+    AdapterSpace w = {};
     auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
+    if (f.rows) {
+        w.bytes = up(M * N * (int64_t)sizeof(float));
+        return w;
+    }
     const int64_t tile_rows = f.pairs ? 2 * BM : BM, n_tiles = (M + tile_rows - 1) / tile_rows;
-    w.tiles = up(f.rows ? M * r * 2 : (n_tiles + S) * tile_rows * r * 2);
-    w.list = w.tiles + (f.rows ? 0 : up(n_tiles * (int64_t)sizeof(int4)));
-    w.bytes = w.list + up((f.rows ? M : n_tiles + S) * (int64_t)sizeof(int));
+    w.tiles = up((n_tiles + S) * tile_rows * r * 2);
+    w.list = w.tiles + up(n_tiles * (int64_t)sizeof(int4));
+    w.bytes = w.list + up((n_tiles + S) * (int64_t)sizeof(int));
     return w;
 }
 
 int64_t adapter_linear_workspace_bytes(int64_t M, int N, int K, int epilogue, int r, int S) {
     if (M <= 0 || S <= 0) return 0;
-    return adapter_space(adapter_form(M, N, K, epilogue == FBB_EPI_SWIGLU, r, S), M, r, S).bytes;
+    return adapter_space(adapter_form(M, N, K, epilogue == FBB_EPI_SWIGLU, r, S), M, N, r, S).bytes;
 }
 
 template <int BN, bool SWIGLU, bool CTA2, AdaptMode ADAPT>
@@ -248,7 +390,7 @@ int launch_adapter_linear(const void* A, const void* W, void* C, const void* bia
                           const int* offsets, int S, void* ws, int64_t ws_bytes, cudaStream_t stream) {
     const bool swiglu = epilogue == FBB_EPI_SWIGLU;
     const AdapterForm f = adapter_form(M, N, K, swiglu, r, S);
-    const AdapterSpace space = adapter_space(f, M, r, S);
+    const AdapterSpace space = adapter_space(f, M, N, r, S);
     if (ws == nullptr || ws_bytes < space.bytes)
         return fail(FBB_ERR_SHAPE, "adapter_linear: workspace of %lld bytes, %lld needed", (long long)(ws != nullptr ? ws_bytes : 0), (long long)space.bytes);
     uint8_t* w8 = reinterpret_cast<uint8_t*>(ws);
@@ -260,21 +402,53 @@ int launch_adapter_linear(const void* A, const void* W, void* C, const void* bia
     d.x = reinterpret_cast<const __half*>(A);
     d.ldx = lda;
     d.down = reinterpret_cast<const __half*>(down);
+    d.up = reinterpret_cast<const __half*>(up);
     d.scale = scale, d.ids = ids, d.offsets = offsets;
-    d.M = (int)M, d.K = K, d.L = L, d.r = r, d.S = S, d.each = offsets != nullptr ? 0 : (int)(M / S);
+    d.M = (int)M, d.N = N, d.K = K, d.L = L, d.r = r, d.S = S, d.each = offsets != nullptr ? 0 : (int)(M / S);
     d.tile_rows = tile_rows;
     d.h = reinterpret_cast<__half*>(ws);
     d.tiles = reinterpret_cast<int4*>(w8 + space.tiles);
     d.list = reinterpret_cast<int*>(w8 + space.list);
+    d.delta = reinterpret_cast<float*>(ws);
+
+    // boxes: 128 rows of A and h, 64 columns of h in the first launch; of W and the adapters' second matrices the rows that one CTA loads
+    // per k-block
+    const uint32_t w_rows = swiglu || f.pairs ? (uint32_t)f.bn / 2 : (uint32_t)f.bn;
+    CUtensorMap ta, tw, th, tu, td, tc;
+    struct { CUtensorMap* map; const void* p; uint64_t cols, rows; int64_t stride; uint32_t box0, box1; CUtensorMapSwizzle swizzle; } maps[6] = {
+        {&ta, A, (uint64_t)K, (uint64_t)M, lda, BK, BM, CU_TENSOR_MAP_SWIZZLE_128B},
+        {&tw, W, (uint64_t)K, (uint64_t)N, ldw, BK, w_rows, CU_TENSOR_MAP_SWIZZLE_128B},
+        {&tc, C, (uint64_t)(swiglu ? N / 2 : N), (uint64_t)M, ldc, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B},
+        {&th, ws, (uint64_t)r, (uint64_t)h_rows, r, BK, BM, CU_TENSOR_MAP_SWIZZLE_128B},
+        {&tu, up, (uint64_t)r, (uint64_t)L * (uint64_t)N, r, BK, w_rows, CU_TENSOR_MAP_SWIZZLE_128B},
+        {&td, down, (uint64_t)K, (uint64_t)L * (uint64_t)r, K, BK, (uint32_t)(r < kDownCols ? r : kDownCols), CU_TENSOR_MAP_SWIZZLE_128B}};
+    for (int i = 0; i < (f.rows ? 3 : 6); ++i) {
+        const uint64_t dims[2] = {maps[i].cols, maps[i].rows};
+        const int64_t st[2] = {1, maps[i].stride};
+        const uint32_t box[2] = {maps[i].box0, maps[i].box1};
+        const int rc = make_tmap_f16(maps[i].map, maps[i].p, 2, dims, st, box, maps[i].swizzle);
+        if (rc != FBB_OK) return rc;
+    }
     cudaError_t e;
     if (f.rows) {
-        e = launch_pdl(adapter_down_rows_kernel, dim3((unsigned)M), dim3(256), 0, stream, d);
+        // enough CTAs to give every SM one, none with fewer columns than threads
+        int64_t parts = (num_sms() + M - 1) / M;
+        parts = parts > (N + 255) / 256 ? (N + 255) / 256 : parts;
+        d.cols = (int)((N + parts - 1) / parts);
+        th = tu = ta;
+        e = launch_pdl(adapter_rows_kernel, dim3((unsigned)M, (unsigned)parts), dim3(256), 0, stream, d);
     } else {
-        const dim3 grid((unsigned)((M + kDownRows - 1) / kDownRows));
-        auto kern = r <= 16 ? adapter_down_blocks_kernel<2> : (r <= 32 ? adapter_down_blocks_kernel<4> : adapter_down_blocks_kernel<8>);
-        e = launch_pdl(kern, grid, dim3(kDownWarps * 32), 0, stream, d);
+        static bool configured[64] = {};
+        int dev = 0;
+        cudaGetDevice(&dev);
+        if (dev < 0 || dev >= 64 || !configured[dev]) {
+            e = cudaFuncSetAttribute(adapter_down_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, DownSmem::kDynamic);
+            if (e != cudaSuccess) return fail((int)e, "cudaFuncSetAttribute(adapter_down_kernel): %s", cudaGetErrorString(e));
+            if (dev >= 0 && dev < 64) configured[dev] = true;
+        }
+        e = launch_pdl(adapter_down_kernel, dim3((unsigned)((M + BM - 1) / BM)), dim3(kDownThreads), DownSmem::kDynamic, stream, ta, td, d);
     }
-    if (e != cudaSuccess) return fail((int)e, "adapter_down kernel launch: %s", cudaGetErrorString(e));
+    if (e != cudaSuccess) return fail((int)e, "adapter kernel launch: %s", cudaGetErrorString(e));
 
     GemmArgs g = {};
     g.C = reinterpret_cast<__half*>(C);
@@ -289,26 +463,10 @@ int launch_adapter_linear(const void* A, const void* W, void* C, const void* bia
     AdaptArgs ad = {};
     ad.tiles = d.tiles;
     ad.list = d.list;
-    ad.h = d.h;
-    ad.up = reinterpret_cast<const __half*>(up);
-    ad.r = r, ad.r_blocks = (r + BK - 1) / BK;
+    ad.delta = d.delta;
+    ad.r_blocks = (r + BK - 1) / BK;
 
-    // boxes: 128 rows of A and h; of W and the adapters' second matrices the rows that one CTA loads per k-block
-    const uint32_t w_rows = swiglu ? (uint32_t)f.bn / 2 : (f.pairs ? (uint32_t)f.bn / 2 : (uint32_t)f.bn);
-    struct { CUtensorMap map; const void* p; uint64_t cols, rows; int64_t stride; uint32_t box0, box1; CUtensorMapSwizzle swizzle; } t[5] = {
-        {{}, A, (uint64_t)K, (uint64_t)M, lda, BK, BM, CU_TENSOR_MAP_SWIZZLE_128B},
-        {{}, W, (uint64_t)K, (uint64_t)N, ldw, BK, w_rows, CU_TENSOR_MAP_SWIZZLE_128B},
-        {{}, f.rows ? A : ws, (uint64_t)(f.rows ? K : r), (uint64_t)(f.rows ? M : h_rows), f.rows ? lda : r, BK, BM, CU_TENSOR_MAP_SWIZZLE_128B},
-        {{}, up, (uint64_t)r, (uint64_t)L * (uint64_t)N, r, BK, w_rows, CU_TENSOR_MAP_SWIZZLE_128B},
-        {{}, C, (uint64_t)g.n_out, (uint64_t)M, ldc, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B}};
-    for (auto& m : t) {
-        const uint64_t dims[2] = {m.cols, m.rows};
-        const int64_t st[2] = {1, m.stride};
-        const uint32_t box[2] = {m.box0, m.box1};
-        const int rc = make_tmap_f16(&m.map, m.p, 2, dims, st, box, m.swizzle);
-        if (rc != FBB_OK) return rc;
-    }
-#define FBB_ADAPTER_LAUNCH(BN, SWIGLU, CTA2, MODE) launch_adapter_variant<BN, SWIGLU, CTA2, MODE>(t[0].map, t[1].map, t[2].map, t[3].map, t[4].map, g, ad, stream)
+#define FBB_ADAPTER_LAUNCH(BN, SWIGLU, CTA2, MODE) launch_adapter_variant<BN, SWIGLU, CTA2, MODE>(ta, tw, th, tu, tc, g, ad, stream)
     if (f.pairs) return swiglu ? FBB_ADAPTER_LAUNCH(256, true, true, kAdaptBlocks) : FBB_ADAPTER_LAUNCH(256, false, true, kAdaptBlocks);
     if (f.rows) {
         if (swiglu) return FBB_ADAPTER_LAUNCH(128, true, false, kAdaptRows);

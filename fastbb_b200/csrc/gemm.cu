@@ -125,13 +125,14 @@ __device__ __forceinline__ void remainder_rows_by_gemv(const GemmArgs& g, bool s
 // What a launch beside the shared projection adds (adapters.cu): of every row tile the products of its requests' adapters.
 enum AdaptMode { kAdaptNone, kAdaptBlocks, kAdaptRows };
 struct AdaptArgs {
-    const int4* tiles;         // blocks: of each row tile {first request, one behind its last, products to add, 0}
-    const int* list;           // blocks: adapter of request s in tile t at t + s, -1: none; rows: of each row
-    const __half* h;           // rows: [M, r], what the adapters' first matrices made of the rows of A, times their scale
-    const __half* up;          // rows: the second matrices [adapters, N, r]
-    const CUtensorMap* map_h;  // blocks: the same per tile and request, [(t + s) * tile rows, r], rows of other requests zero
-    const CUtensorMap* map_up;
-    int r, r_blocks;           // rank, and the 64-element k-blocks it takes
+    // blocks
+    const int4* tiles;         // of each row tile {first request, one behind its last, products to add, 0}
+    const int* list;           // adapter of request s in tile t at t + s, -1: none
+    const CUtensorMap* map_h;  // h of request s in tile t from row (t + s) * tile rows on, rows of other requests zero
+    const CUtensorMap* map_up; // the adapters' second matrices [adapters * N, r]
+    int r_blocks;              // 64-element k-blocks of the rank
+    // rows
+    const float* delta;        // [M, N]: added to the accumulator
 };
 
 template <int BN, bool SWIGLU, bool CTA2, bool SLICES, AdaptMode ADAPT>
@@ -363,35 +364,18 @@ __device__ __forceinline__ void linear_umma_body(const CUtensorMap& tmap_a, cons
                     }
                 }
             }
-            // This thread's row of h times the rows of its adapter's second matrix that belong to columns n .. n + 31, on the CUDA cores:
-            // where requests have few rows, a k-block per request and tile costs more.
-            int slot = -1;
-            if constexpr (ADAPT == kAdaptRows) {
-                grid_dependency_wait();
-                if (row_ok) slot = __ldcg(ad.list + row);
-            }
-            auto add_adapter = [&](float* v, int n) {
-                if (slot < 0) return;
-                const uint4* hr = reinterpret_cast<const uint4*>(ad.h + (int64_t)row * ad.r);
-                const uint4* up = reinterpret_cast<const uint4*>(ad.up + (int64_t)slot * g.N * ad.r);
-                const int vecs = ad.r >> 3;  // a row's 16-byte vectors
-                for (int p = 0; p < vecs; ++p) {
-                    const uint4 hv = __ldcg(hr + p);
-                    const __half2* hh = reinterpret_cast<const __half2*>(&hv);
-                    float2 hf[4];
+            // what the adapters add to this thread's row, columns n .. n + 31
+            auto add_delta = [&](float* v, int n) {
+                if (!row_ok) return;
+                const float4* d = reinterpret_cast<const float4*>(ad.delta + (int64_t)row * g.N + n);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) hf[e] = __half22float2(hh[e]);
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        const uint4 uv = __ldg(up + (int64_t)min(n + j, g.N - 1) * vecs + p);  // (a column beyond the last is not stored)
-                        const __half2* uh = reinterpret_cast<const __half2*>(&uv);
-                        float2 sum = make_float2(v[j], 0.f);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) sum = ffma2(hf[e], __half22float2(uh[e]), sum);
-                        v[j] = sum.x + sum.y;
-                    }
+                for (int j = 0; j < 8; ++j) {
+                    if (n + 4 * j >= g.N) break;
+                    const float4 x = __ldcg(d + j);
+                    v[4 * j] += x.x, v[4 * j + 1] += x.y, v[4 * j + 2] += x.z, v[4 * j + 3] += x.w;
                 }
             };
+            if constexpr (ADAPT == kAdaptRows) grid_dependency_wait();
             if (!mbar_wait(tfull_bar(acc), acc_ph, s_abort, DEV_TIMEOUT_TMEM_FULL, acc)) break;
             tc_fence_after();
             const uint32_t t_row = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * BN);
@@ -410,7 +394,7 @@ __device__ __forceinline__ void linear_umma_body(const CUtensorMap& tmap_a, cons
 #pragma unroll
                     for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
                 }
-                if constexpr (ADAPT == kAdaptRows) add_adapter(v, n0 + c0);
+                if constexpr (ADAPT == kAdaptRows) add_delta(v, n0 + c0);
                 if (SWIGLU) {
                     uint32_t r2[32];
                     tmem_ld32(t_row + (uint32_t)(BN / 2 + c0), r2);
@@ -419,7 +403,7 @@ __device__ __forceinline__ void linear_umma_body(const CUtensorMap& tmap_a, cons
                         float v2[32];
 #pragma unroll
                         for (int j = 0; j < 32; ++j) v2[j] = __uint_as_float(r2[j]);
-                        add_adapter(v2, g.N / 2 + n0 + c0);
+                        add_delta(v2, g.N / 2 + n0 + c0);
 #pragma unroll
                         for (int j = 0; j < 32; ++j) r2[j] = __float_as_uint(v2[j]);
                     }
