@@ -28,7 +28,7 @@
 namespace fbb {
 
 constexpr int kDiffStages = 3;
-constexpr int kDiffRowValues = 68;  // of a lane in a 16-row group of one map: 64 outputs, two maxima, two sums, in fours per lane
+constexpr int kDiffPart = 16 * 128 + 16 * 2;  // floats of 16 rows of a share and map: the outputs, then {maximum, sum} of each row
 
 struct DiffSmem {
     static constexpr int kQOff = 0;                       // Q_1 | Q_2
@@ -53,7 +53,7 @@ struct DiffArgs {
     const int* lengths;      // keys of each batch entry, null: Nk
     int B, H, group;         // group = query heads per key head
     int Nq, Nk, q_tiles, splits;
-    float* part;             // [tile][split][map][16-row group][kDiffRowValues / 4][32][4], null when splits == 1
+    float* part;             // [tile][split][map][16-row group][kDiffPart], null when splits == 1
     int row_groups;          // of a tile that hold rows: min(8, ceil(Nq / 16))
 };
 
@@ -352,17 +352,22 @@ diff64_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
             if (a.splits > 1) {
                 // the rows of this share for diff64_join_kernel (which asks for no share without keys)
                 if (halves > 0) {
-                    float4* dst = reinterpret_cast<float4*>(a.part + ((((int64_t)blockIdx.x * 2 + t) * a.row_groups + (lane_base >> 4)) * kDiffRowValues) * 32) + lane;
+                    float* dst = a.part + (((int64_t)blockIdx.x * 2 + t) * a.row_groups + (lane_base >> 4)) * kDiffPart;
+                    float2* outA = reinterpret_cast<float2*>(dst + (lane >> 2) * 128 + 2 * cq);
 #pragma unroll 1
                     for (int c = 0; c < 8; ++c) {
                         uint32_t o[8];
                         tmem_ld_16x256b_x2(tO + 16u * c, o);
                         tmem_wait_ld();
 #pragma unroll
-                        for (int i = 0; i < 2; ++i)
-                            dst[(2 * c + i) * 32] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+                        for (int i = 0; i < 2; ++i) {
+                            outA[8 * c + 4 * i] = make_float2(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]));
+                            outA[8 * c + 4 * i + 8 * 64] = make_float2(__uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));  // row B
+                        }
                     }
-                    dst[16 * 32] = make_float4(mA, mB, lA, lB);
+                    float2* stat = reinterpret_cast<float2*>(dst + 16 * 128);
+                    if (cq == 0) stat[lane >> 2] = make_float2(mA, lA);
+                    if (cq == 1) stat[(lane >> 2) + 8] = make_float2(mB, lB);
                 }
             } else {
                 // Map 1's warps leave lam O_2 / l_2 in shared memory, where their twins of map 0, which hold the same elements of O_1, take it:
@@ -447,113 +452,101 @@ diff64_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
 }
 
 // Joins the shares of a 16-row group's keys: a share's weight is 2^(its maximum - the row's) over the row's sum. A chain of latencies (the
-// partial rows are a few hundred KB in L2), so what does not depend on anything is loaded at once: every share's maxima and sums by
-// one thread each, the first shares' outputs ahead of the weights. 16 warps: eight eighths of the 64 values of each map; then 16 threads per
-// row take the difference, the norm and the store.
+// partial rows are a few hundred KB in L2): what does not depend on anything is loaded at once, every share's maxima and sums by one
+// thread each and the first shares' outputs ahead of the weights. Thread = (map, row, eight columns); those of rows beyond Nq rest.
 constexpr int kDiffMaxSplits = 160;
 constexpr int kJoinBatch = 8;
 __global__ void __launch_bounds__(512) diff64_join_kernel(const DiffArgs a) {
-    __shared__ float s_weight[kDiffMaxSplits][2][16];  // [share][map][row]: the maximum, then the weight
-    __shared__ __align__(16) float s_both[kDiffMaxSplits * 32];
-    static_assert(kDiffMaxSplits * 32 >= 2 * 16 * 132, "the outputs take the place of the sums");
-    auto s_sum = reinterpret_cast<float(*)[2][16]>(s_both);
-    auto s_o = reinterpret_cast<float(*)[16][132]>(s_both);  // [map][row][column], once the sums are used up; rows 4 banks apart
+    __shared__ float2 s_stat[kDiffMaxSplits][2][16];  // [share][map][row]: {maximum, sum}, then {weight, -}
+    __shared__ __align__(16) float s_o[16][128];      // map 1's rows
+    const unsigned tile = blockIdx.x / (unsigned)a.row_groups, rg = blockIdx.x - tile * (unsigned)a.row_groups;
+    const unsigned bh = tile / (unsigned)a.q_tiles;
+    const int row0 = (int)(tile - bh * (unsigned)a.q_tiles) * FQ + (int)rg * 16;
+    const int b = (int)(bh / (unsigned)a.H), h = (int)bh - b * a.H;
+    const int t = threadIdx.x >> 8, r = (threadIdx.x >> 4) & 15, c = (threadIdx.x & 15) * 8, strand = threadIdx.x & 15;
     grid_dependency_wait();
     grid_launch_dependents();
-    const int tile = (int)(blockIdx.x / (unsigned)a.row_groups), rg = (int)blockIdx.x - tile * a.row_groups;
-    const int bh = (int)((unsigned)tile / (unsigned)a.q_tiles), row0 = (tile - bh * a.q_tiles) * FQ + rg * 16;
-    const int b = (int)((unsigned)bh / (unsigned)a.H), h = bh - b * a.H;
     if (row0 >= a.Nq) return;
+    const bool used = row0 + r < a.Nq;
     const int keys = diff_keys(a, b);
-    const int64_t step = (int64_t)2 * a.row_groups * (kDiffRowValues / 4) * 32;  // float4s from share to share, from map to map half of it
-    const float4* part = reinterpret_cast<const float4*>(a.part) + (int64_t)tile * a.splits * step + (int64_t)rg * (kDiffRowValues / 4) * 32;
+    const int step = 2 * a.row_groups * kDiffPart;  // floats from share to share, from map to map half of it
+    const float* part = a.part + (int64_t)tile * a.splits * step + (int64_t)rg * kDiffPart;
     // the shares that hold keys: all of them, or as many as there are blocks
-    const int blocks = (keys + FK - 1) / FK, live = min(blocks, a.splits);
+    const int blocks = (int)(((unsigned)keys + FK - 1) / FK), live = min(blocks, a.splits);
     auto share = [&](int j) { return blocks >= a.splits ? j : (int)(((unsigned)(j + 1) * (unsigned)a.splits + (unsigned)blocks - 1u) / (unsigned)blocks) - 1; };
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int t = warp >> 3, v0 = (warp & 7) * 8;  // this warp's map and values
-    const int rA = lane >> 2, rB = rA + 8;
-    const bool used = row0 + rA < a.Nq;            // (row B only if row A)
-    const float4* src = part + t * (step / 2) + (v0 / 4) * 32 + lane;
+    const float* src = part + t * (step / 2) + r * 128 + c;
     float4 x[kJoinBatch][2];
     auto load = [&](int j0) {
 #pragma unroll
         for (int j = 0; j < kJoinBatch; ++j) {
-            if (!used || j0 + j >= live) continue;
-            x[j][0] = __ldcg(src + share(j0 + j) * step);
-            x[j][1] = __ldcg(src + share(j0 + j) * step + 32);
+            if (j0 + j >= live) break;
+            const float4* at = reinterpret_cast<const float4*>(src + (int64_t)share(j0 + j) * step);
+            x[j][0] = __ldcg(at);
+            x[j][1] = __ldcg(at + 1);
         }
     };
-    load(0);
-    // the final threads' factors: row threadIdx.x / 16 of the lower 256 threads, columns fc ..
-    const int fr = threadIdx.x >> 4, fc = (threadIdx.x & 15) * 8;
-    const bool final_thread = threadIdx.x < 256 && row0 + fr < a.Nq;
-    float factor[8] = {1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
-    if (final_thread && a.weight != nullptr) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) factor[i] = diff_weight(a, fc + i);
-    }
-    const int pair = threadIdx.x >> 4, strand = threadIdx.x & 15, pt = pair >> 4, pr = pair & 15;  // (map, row), one of 16 strands of the shares
+    if (used) load(0);
     float lam = 1.f;
-    if (pt == 1) lam = row0 + pr < a.Nq ? a.lam[b * a.l_sb + (row0 + pr) * a.l_sn + h * a.l_sh] : 0.f;
-    for (int i = threadIdx.x; i < live * 16; i += 512) {
-        const int j = i >> 4, mt = (i >> 3) & 1, q = i & 7;  // a share's map, rows q and q + 8
-        const float4 st = __ldcg(part + share(j) * step + mt * (step / 2) + 16 * 32 + 4 * q);
-        s_weight[j][mt][q] = st.x, s_weight[j][mt][q + 8] = st.y;
-        s_sum[j][mt][q] = st.z, s_sum[j][mt][q + 8] = st.w;
+    if (t == 1 && used) lam = a.lam[b * a.l_sb + (row0 + r) * a.l_sn + h * a.l_sh];
+    for (int i = threadIdx.x; i < live * 32; i += 512) {
+        const int j = i >> 5, mr = i & 31;
+        s_stat[j][mr >> 4][mr & 15] = __ldcg(reinterpret_cast<const float2*>(part + (int64_t)share(j) * step + (mr >> 4) * (step / 2) + 16 * 128) + (mr & 15));
     }
     __syncthreads();
-    {
+    if (used) {  // (whole rows of 16 threads, whose shuffles stay among themselves)
+        const unsigned mask = 0xffffu << (threadIdx.x & 16);
         float m = -INFINITY, l = 0.f;
-        for (int j = strand; j < live; j += 16) m = fmaxf(m, s_weight[j][pt][pr]);
+        for (int j = strand; j < live; j += 16) m = fmaxf(m, s_stat[j][t][r].x);
 #pragma unroll
-        for (int d = 1; d < 16; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-        for (int j = strand; j < live; j += 16) l = fmaf(ex2_approx(s_weight[j][pt][pr] - m), s_sum[j][pt][pr], l);
+        for (int d = 1; d < 16; d <<= 1) m = fmaxf(m, __shfl_xor_sync(mask, m, d));
+        for (int j = strand; j < live; j += 16) {
+            const float w = ex2_approx(s_stat[j][t][r].x - m);
+            l = fmaf(w, s_stat[j][t][r].y, l);
+            s_stat[j][t][r].x = w;
+        }
 #pragma unroll
-        for (int d = 1; d < 16; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+        for (int d = 1; d < 16; d <<= 1) l += __shfl_xor_sync(mask, l, d);
         const float f = lam / l;
-        for (int j = strand; j < live; j += 16) s_weight[j][pt][pr] = ex2_approx(s_weight[j][pt][pr] - m) * f;
-    }
-    __syncthreads();
-    float acc[8] = {};
-    for (int j0 = 0; j0 < live; j0 += kJoinBatch) {
-        if (j0 > 0) load(j0);
+        __syncwarp(mask);
+        float acc[8] = {};
+        for (int j0 = 0; j0 < live; j0 += kJoinBatch) {
+            if (j0 > 0) load(j0);
 #pragma unroll
-        for (int j = 0; j < kJoinBatch; ++j) {
-            if (!used || j0 + j >= live) continue;
-            const float wA = s_weight[j0 + j][t][rA], wB = s_weight[j0 + j][t][rB];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                acc[4 * i] = fmaf(x[j][i].x, wA, acc[4 * i]);
-                acc[4 * i + 1] = fmaf(x[j][i].y, wA, acc[4 * i + 1]);
-                acc[4 * i + 2] = fmaf(x[j][i].z, wB, acc[4 * i + 2]);
-                acc[4 * i + 3] = fmaf(x[j][i].w, wB, acc[4 * i + 3]);
+            for (int j = 0; j < kJoinBatch; ++j) {
+                if (j0 + j >= live) break;
+                const float w = s_stat[j0 + j][t][r].x;
+                acc[0] = fmaf(x[j][0].x, w, acc[0]), acc[1] = fmaf(x[j][0].y, w, acc[1]), acc[2] = fmaf(x[j][0].z, w, acc[2]), acc[3] = fmaf(x[j][0].w, w, acc[3]);
+                acc[4] = fmaf(x[j][1].x, w, acc[4]), acc[5] = fmaf(x[j][1].y, w, acc[5]), acc[6] = fmaf(x[j][1].z, w, acc[6]), acc[7] = fmaf(x[j][1].w, w, acc[7]);
             }
         }
-    }
 #pragma unroll
-    for (int i = 0; i < 8; i += 2)
-        *reinterpret_cast<float2*>(&s_o[t][(i & 2) ? rB : rA][8 * ((v0 + i) >> 2) + 2 * (lane & 3)]) = make_float2(acc[i], acc[i + 1]);
+        for (int i = 0; i < 8; ++i) acc[i] = live > 0 ? acc[i] * f : 0.f;
+        if (t == 1) {
+            *reinterpret_cast<float4*>(&s_o[r][c]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+            *reinterpret_cast<float4*>(&s_o[r][c + 4]) = make_float4(acc[4], acc[5], acc[6], acc[7]);
+        }
+        x[0][0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+        x[0][1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+    }
     __syncthreads();
-    if (threadIdx.x >= 256) return;
-    float o[8], sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        o[i] = s_o[0][fr][fc + i] - s_o[1][fr][fc + i];
-        sum = fmaf(o[i], o[i], sum);
-    }
+    if (t == 1 || !used) return;
+    const float4 y0 = *reinterpret_cast<const float4*>(&s_o[r][c]), y1 = *reinterpret_cast<const float4*>(&s_o[r][c + 4]);
+    float o[8] = {x[0][0].x - y0.x, x[0][0].y - y0.y, x[0][0].z - y0.z, x[0][0].w - y0.w, x[0][1].x - y1.x, x[0][1].y - y1.y, x[0][1].z - y1.z, x[0][1].w - y1.w};
     float scale = a.out_scale;
     if (a.weight != nullptr) {
+        const unsigned mask = 0xffffu << (threadIdx.x & 16);
+        float sum = 0.f;
 #pragma unroll
-        for (int d = 1; d < 16; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        for (int i = 0; i < 8; ++i) sum = fmaf(o[i], o[i], sum);
+#pragma unroll
+        for (int d = 1; d < 16; d <<= 1) sum += __shfl_xor_sync(mask, sum, d);
         scale *= rsqrtf(sum * (1.f / 128.f) + a.eps);
-    }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] *= scale * factor[i];
-    if (final_thread)
-        *reinterpret_cast<uint4*>(a.o + b * a.o_sb + (int64_t)(row0 + fr) * a.o_sn + h * a.o_sh + fc) =
-            make_uint4(pack_h2(o[0], o[1]), pack_h2(o[2], o[3]), pack_h2(o[4], o[5]), pack_h2(o[6], o[7]));
+        for (int i = 0; i < 8; ++i) o[i] *= diff_weight(a, c + i);
+    }
+    *reinterpret_cast<uint4*>(a.o + b * a.o_sb + (int64_t)(row0 + r) * a.o_sn + h * a.o_sh + c) =
+        make_uint4(pack_h2(o[0] * scale, o[1] * scale), pack_h2(o[2] * scale, o[3] * scale), pack_h2(o[4] * scale, o[5] * scale), pack_h2(o[6] * scale, o[7] * scale));
 }
 
 // Shares of the keys: as many as fill the SMs once, none of less than two blocks.
@@ -570,7 +563,7 @@ int64_t diff64_workspace_bytes(int B, int Nq, int Nk, int H) {
     if (B <= 0 || Nq <= 0 || H <= 0) return 0;
     const int splits = diff64_splits(B, Nq, Nk, H);
     if (splits == 1) return 0;
-    return (int64_t)B * H * ((Nq + FQ - 1) / FQ) * splits * 2 * diff64_row_groups(Nq) * kDiffRowValues * 32 * (int64_t)sizeof(float);
+    return (int64_t)B * H * ((Nq + FQ - 1) / FQ) * splits * 2 * diff64_row_groups(Nq) * kDiffPart * (int64_t)sizeof(float);
 }
 int diff64_launches(int B, int Nq, int Nk, int H) { return B > 0 && Nq > 0 && H > 0 ? (diff64_splits(B, Nq, Nk, H) > 1 ? 2 : 1) : 0; }
 
