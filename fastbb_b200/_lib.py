@@ -148,44 +148,51 @@ def ptr(t):
 
 
 def _nested(t):
-    """(size, stride) of t's dimensions of more than one element, innermost first, and whether no two elements share an address
+    """(stride, size) of t's dimensions of more than one element, innermost first, and whether no two elements share an address
     (every stride steps over what the dimensions inside it span)."""
-    dims = sorted(((n, s) for n, s in zip(t.shape, t.stride()) if n > 1), key=lambda d: d[1])
-    span, ok = 1, True
-    for n, s in dims:
-        ok = ok and s >= span
+    dims = sorted([(s, n) for n, s in zip(t.shape, t.stride()) if n > 1])
+    span = 1
+    for s, n in dims:
+        if s < span:
+            return dims, False
         span += (n - 1) * s
-    return dims, ok
+    return dims, True
 
 
 def writable(t):
     """Whether every element of t has an address of its own (an expanded or self-overlapping view cannot be written by many threads)."""
-    return t.numel() == 0 or _nested(t)[1]
+    return t.is_contiguous() or t.numel() == 0 or _nested(t)[1]
 
 
 def same_view(a, b):
-    return a.data_ptr() == b.data_ptr() and a.shape == b.shape and a.dtype == b.dtype and all(
-        n == 1 or s == r for n, s, r in zip(a.shape, a.stride(), b.stride()))
+    return a is b or (a.data_ptr() == b.data_ptr() and a.shape == b.shape and a.dtype == b.dtype and all(
+        n == 1 or s == r for n, s, r in zip(a.shape, a.stride(), b.stride())))
 
 
 def disjoint(a, b):
-    """Whether a and b (of one dtype) surely share no element: other storages, byte ranges apart, or views of one buffer that lie beside
-    each other within equal outer strides, like the queries and keys of a packed projection."""
-    if a.numel() == 0 or b.numel() == 0 or a.untyped_storage().data_ptr() != b.untyped_storage().data_ptr():
+    """Whether a and b (of one dtype) surely share no element: byte ranges apart, or views of one buffer that lie beside each other
+    within equal outer strides, like the queries and keys of a packed projection."""
+    pa, pb = a.data_ptr(), b.data_ptr()
+    if pa > pb:
+        a, b, pa, pb = b, a, pb, pa
+    size = a.element_size()
+    if pb - pa >= size * a.numel() and a.is_contiguous():
         return True
-    if a.data_ptr() > b.data_ptr():
-        a, b = b, a
-    gap = (b.data_ptr() - a.data_ptr()) // a.element_size()
+    if a.numel() == 0 or b.numel() == 0:
+        return True
+    gap = (pb - pa) // size
     da, db = _nested(a)[0], _nested(b)[0]
-    for k in range(len(da) + 1):  # the k innermost dimensions of a against what the outer ones leave for b
+    if gap > sum([(n - 1) * s for s, n in da]):
+        return True
+    for k in range(len(da)):  # the k innermost dimensions of a against what the next one leaves for b
         outer = da[k:]
         m = len(db) - len(outer)
         if m < 0 or db[m:] != outer:
             continue
-        span_a, span_b = 1 + sum((n - 1) * s for n, s in da[:k]), 1 + sum((n - 1) * s for n, s in db[:m])
-        if gap >= span_a and (not outer or gap + span_b <= outer[0][1]):
+        span_a, span_b = 1 + sum([(n - 1) * s for s, n in da[:k]]), 1 + sum([(n - 1) * s for s, n in db[:m]])
+        if gap >= span_a and gap + span_b <= outer[0][0]:
             return True
-    return 1 + sum((n - 1) * s for n, s in da) <= gap
+    return False
 
 
 def device_status():

@@ -74,33 +74,38 @@ def adapter_linear(x, w, adapters, ids, offsets=None, b=None, act=None, res=None
     if gamma is not None and res is None:
         raise ValueError("gamma is the LayerScale of the residual epilogue: it needs res")
     if out is None:
-        out = torch.empty(oshape, device=device, dtype=torch.float16)
+        out = x.new_empty(oshape)
     else:
         if out.shape != oshape or out.device != device or out.dtype != torch.float16 or not out.is_contiguous() or out.data_ptr() % 16:
             raise ValueError("out must be contiguous with the output shape, input dtype and device")
         if not (_lib.disjoint(out, x) and _lib.disjoint(out, w) and (res is None or _lib.same_view(out, res) or _lib.disjoint(out, res))):
             raise ValueError("out may be res itself and shares no memory with the other inputs")
-    x2 = x.reshape(-1, K)
-    if x2.stride(-1) != 1:
-        x2 = x2.contiguous()
+    if x.is_contiguous():
+        x2, lda = x, K
+    else:
+        x2 = x.reshape(-1, K)
+        if x2.stride(-1) != 1:
+            x2 = x2.contiguous()
+        lda = x2.stride(0) if x2.shape[0] > 1 else K
     if w.stride(-1) != 1:
         w = w.contiguous()
-    r2 = None
-    if res is not None:
+    r2, ldr = res, n_out
+    if res is not None and not res.is_contiguous():
         r2 = res.reshape(-1, n_out)
         if r2.stride(-1) != 1:
             r2 = r2.contiguous()
-    M = x2.shape[0]
+        ldr = r2.stride(0) if r2.shape[0] > 1 else n_out
+    M = x.numel() // K if K else 0
     if M == 0:
         return out
     code = _ACT[act]
     with _lib.on(device):
         lib = _lib.load()
         need = lib.fbb_adapter_linear_workspace_bytes(M, N, K, code, adapters.rank, S)
-        ws = torch.empty(need, device=device, dtype=torch.uint8)
+        ws = x.new_empty((need + 1) // 2)
         _lib.check(lib.fbb_adapter_linear_f16(
-            x2.data_ptr(), w.data_ptr(), out.data_ptr(), _lib.ptr(b), _lib.ptr(r2), _lib.ptr(gamma), M, N, K, x2.stride(0) if M > 1 else K,
-            w.stride(0) if N > 1 else K, n_out, (r2.stride(0) if M > 1 else n_out) if r2 is not None else 0, code, adapters.down.data_ptr(),
+            x2.data_ptr(), w.data_ptr(), out.data_ptr(), _lib.ptr(b), _lib.ptr(r2), _lib.ptr(gamma), M, N, K, lda,
+            w.stride(0) if N > 1 else K, n_out, ldr if res is not None else 0, code, adapters.down.data_ptr(),
             adapters.up.data_ptr(), adapters.scale.data_ptr(), adapters.count, adapters.rank, ids.data_ptr(), _lib.ptr(offsets), S, ws.data_ptr(), need,
             _lib.stream_ptr(device)))
         _lib.launched(2)

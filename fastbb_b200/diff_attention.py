@@ -12,8 +12,14 @@ from . import _lib
 
 
 def _usable(t, columns):
-    return (t.is_cuda and t.dtype == torch.float16 and t.dim() == 4 and t.shape[3] == columns and t.stride(3) == 1 and t.data_ptr() % 16 == 0
-            and all(n <= 1 or (s % 8 == 0 and s > 0) for n, s in zip(t.shape[:3], t.stride())))
+    """(shape, stride, address) of a view that the kernel takes, None of any other."""
+    shape, stride, ptr = t.shape, t.stride(), t.data_ptr()
+    if not t.is_cuda or t.dtype is not torch.float16 or len(shape) != 4 or shape[3] != columns or stride[3] != 1 or ptr & 15:
+        return None
+    a, b, c, _ = stride
+    if ((a | b | c) & 7 or not (a and b and c)) and not all(n <= 1 or (s % 8 == 0 and s > 0) for n, s in zip(shape[:3], stride)):
+        return None
+    return shape, stride, ptr
 
 
 def diff_attention(q, k, v, lam, weight=None, eps=1e-5, out_scale=1.0, scale=None, key_lengths=None, out=None):
@@ -26,13 +32,15 @@ def diff_attention(q, k, v, lam, weight=None, eps=1e-5, out_scale=1.0, scale=Non
     out_scale: a factor of the result, with or without the norm. scale: of the scores, 64^-0.5 unless given, > 0.
     key_lengths: int32 [B] on the GPU: keys from key_lengths[b] on are not seen, whatever they hold; a row without keys is 0.
     out: fp16 [B, Nq, H, 128] that shares no memory with the inputs."""
-    if not (_usable(q, 64) and _usable(k, 64) and _usable(v, 128)):
+    uq, uk, uv = _usable(q, 64), _usable(k, 64), _usable(v, 128)
+    if uq is None or uk is None or uv is None:
         raise ValueError("diff_attention needs CUDA fp16 q, k [B, N, 2 * heads, 64] and v [B, N, heads, 128] with a contiguous last dim, other strides "
                          "that are multiples of 8 elements and 16-byte aligned storage (there is no fallback path)")
-    B, Nq, H2, _ = q.shape
-    _, Nk, Hk, _ = v.shape
+    (B, Nq, H2, _), qs, q_ptr = uq
+    (Bk, Nk, Hk2, _), ks, k_ptr = uk
+    (Bv, Nv, Hk, _), vs, v_ptr = uv
     H, device = H2 // 2, q.device
-    if k.device != device or v.device != device or k.shape != (B, Nk, 2 * Hk, 64) or v.shape[0] != B or H2 % 2 or Hk == 0 or H == 0 or H % Hk:
+    if k.device != device or v.device != device or Bk != B or Bv != B or Nv != Nk or Hk2 != 2 * Hk or H2 % 2 or Hk == 0 or H == 0 or H % Hk:
         raise ValueError("q must be [B, Nq, 2H, 64], k [B, Nk, 2Hk, 64] and v [B, Nk, Hk, 128] on one device, Hk a divisor of H")
     if scale is None:
         scale = 0.125
@@ -40,18 +48,21 @@ def diff_attention(q, k, v, lam, weight=None, eps=1e-5, out_scale=1.0, scale=Non
         raise ValueError("scale must be > 0 and eps >= 0")
     if not torch.is_tensor(lam) or lam.dtype != torch.float32 or lam.device != device:
         raise ValueError("lam must be an fp32 tensor on the inputs' device")
-    try:
-        lam = lam.expand(B, Nq, H)
-    except RuntimeError:
-        raise ValueError(f"lam must broadcast to {(B, Nq, H)}, got {tuple(lam.shape)}") from None
+    if lam.dim() == 1 and lam.shape[0] == H:
+        ls = (0, 0, lam.stride(0))
+    else:
+        try:
+            ls = lam.expand(B, Nq, H).stride()
+        except RuntimeError:
+            raise ValueError(f"lam must broadcast to {(B, Nq, H)}, got {tuple(lam.shape)}") from None
     if weight is not None and (weight.device != device or weight.dtype not in (torch.float16, torch.float32) or weight.shape != (128,) or not weight.is_contiguous()):
         raise ValueError("weight must be a contiguous fp16 or fp32 vector of 128 on the inputs' device")
     if key_lengths is not None and (key_lengths.device != device or key_lengths.dtype != torch.int32 or key_lengths.shape != (B,)
                                     or not key_lengths.is_contiguous()):
         raise ValueError(f"key_lengths must be a contiguous int32 vector of {B} on the inputs' device")
     if out is None:
-        out = torch.empty((B, Nq, H, 128), device=device, dtype=torch.float16)
-    elif not (_usable(out, 128) and out.shape == (B, Nq, H, 128) and out.device == device and _lib.writable(out)):
+        out = q.new_empty((B, Nq, H, 128))
+    elif not (_usable(out, 128) is not None and out.shape == (B, Nq, H, 128) and out.device == device and _lib.writable(out)):
         raise ValueError("out must be fp16 [B, Nq, H, 128] on the inputs' device, with a contiguous last dim, strides that are multiples of 8 elements, "
                          "16-byte aligned and no element twice")
     elif not (_lib.disjoint(out, q) and _lib.disjoint(out, k) and _lib.disjoint(out, v)):
@@ -61,10 +72,9 @@ def diff_attention(q, k, v, lam, weight=None, eps=1e-5, out_scale=1.0, scale=Non
     with _lib.on(device):
         lib = _lib.load()
         need = lib.fbb_diff64_workspace_bytes(B, Nq, Nk, H)
-        ws = torch.empty(need, device=device, dtype=torch.uint8) if need > 0 else None
+        ws = q.new_empty((need + 1) // 2) if need > 0 else None
         _lib.check(lib.fbb_diff64_f16(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), B, Nq, Nk, H, Hk, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3],
-            lam.data_ptr(), *lam.stride(), _lib.ptr(weight), _lib.DTYPE_CODE[weight.dtype] if weight is not None else 0, float(eps), float(out_scale),
+            q_ptr, k_ptr, v_ptr, out.data_ptr(), B, Nq, Nk, H, Hk, *qs[:3], *ks[:3], *vs[:3], *out.stride()[:3], lam.data_ptr(), *ls, _lib.ptr(weight), _lib.DTYPE_CODE[weight.dtype] if weight is not None else 0, float(eps), float(out_scale),
             float(scale), _lib.ptr(key_lengths), _lib.ptr(ws), need, _lib.stream_ptr(device)))
         _lib.launched(lib.fbb_diff64_launches(B, Nq, Nk, H))
     return out

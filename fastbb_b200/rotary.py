@@ -110,7 +110,8 @@ def rotary(q, k, positions, plan, n_prefix=0, inverse=False, out=None):
     if len(pos_shape) == 2:
         pos_strides = (0, *pos_strides)
     if out is None:
-        result = torch.empty(shape, device=device, dtype=dtype), torch.empty(k_shape, device=device, dtype=dtype) if k is not None else None
+        result = (torch.empty_like(q, memory_format=torch.contiguous_format),
+                  torch.empty_like(k, memory_format=torch.contiguous_format) if k is not None else None)
     else:
         result = _checked(out, q, k)
     if B == 0 or N == 0:
@@ -137,10 +138,11 @@ def _checked(out, q, k):
     if len(outs) != len(inputs):
         raise ValueError("out must be a pair (q_out, k_out)")
     for i, y in enumerate(outs):
-        if y.shape != inputs[i].shape or y.dtype != q.dtype or y.device != q.device or (y.stride(3) != 1 and y.shape[3] > 1) or not _lib.writable(y):
+        x = inputs[i]
+        if y is not x and (y.shape != x.shape or y.dtype != q.dtype or y.device != q.device or (y.stride(3) != 1 and y.shape[3] > 1)) or not _lib.writable(y):
             raise ValueError("out must match the inputs' shapes, dtype and device, with a contiguous last dim and no element twice")
-        if not all(_lib.disjoint(y, x) or (i == j and _lib.same_view(y, x)) for j, x in enumerate(inputs)):
+        if not (_lib.same_view(y, x) or _lib.disjoint(y, x)) or (k is not None and not _lib.disjoint(y, inputs[1 - i])):
             raise ValueError("out must be its own input or share no memory with the inputs")
-    if len(outs) == 2 and not _lib.disjoint(*outs):
+    if len(outs) == 2 and (outs[0] is not q or outs[1] is not k) and not _lib.disjoint(*outs):
         raise ValueError("the two outputs share memory")
     return outs[0], outs[1] if k is not None else None
