@@ -1,9 +1,11 @@
 // Differential attention: o = softmax(scale q1 k1') v - lam softmax(scale q2 k2') v, two maps of head dimension 64 over the same
 // values of 128 columns, and the root-mean-square norm of every head's row behind it. No mask but a number of keys per batch entry.
 //
-// One CTA takes 128 queries of one (batch, head) and walks its keys in blocks of 128, both maps at once, so that v is read once and
-// no map or half of an output ever leaves the chip (as four calls of the flash64 kernel, one per map and half of v, every score is
-// computed twice and three passes over the outputs follow).
+// A tile is 128 queries of one (batch, head); it walks its keys in blocks of 128, both maps at once, so that v is read once and no map
+// or half of an output ever leaves the chip (as four calls of the flash64 kernel, one per map and half of v, every score is computed
+// twice and three passes over the outputs follow). One persistent CTA per SM takes every so-manieth tile. Where the tiles are fewer than
+// the SMs (few queries over many keys), each is split over the keys instead, and the splits' unnormalised rows, maxima and sums go
+// through the workspace to diff64_join_kernel.
 //   warp 0          TMA producer: the two Q tiles, then K1, K2 and V of each block into a ring of stages (128-byte swizzle)
 //   warps 1, 2      UMMA issuers, one per map: S_t = Q_t K_t^T of half a block (64 keys) into one of two halves of the map's tensor memory;
 //                   once the softmax warps have put P_t (fp16) over it, O_t += P_t V (A from tensor memory, V as the MN-major B
@@ -17,28 +19,30 @@
 // S of a whole block per map, its exponentials and its products took turns (3700 clocks per block and both maps); in halves, one half's
 // P.V and the scores after it run under the other half's exponentials.
 //
-// Few queries over many keys (fewer tiles than SMs): the keys are split over `splits` CTAs, each of which leaves its unnormalised rows,
-// maxima and sums in the workspace for diff64_join_kernel. Keys beyond a batch entry's number are masked by selection, never by
-// adding, and their rows of V are zeroed in shared memory ahead of the product, so that no infinity or NaN in them is seen.
-#include <type_traits>
-
+// The next item's Q, K and first scores are on their way while the softmax warps finish the last one; only its first P.V waits for them
+// to have read O. Map 0's and map 1's warps of the same rows finish a tile together, half of the columns each: both read O_1 and O_2.
+//
+// Keys beyond a batch entry's number are masked by selection, never by adding, and their rows of V are zeroed in shared memory ahead
+// of the product, so that no infinity or NaN in them is seen.
 #include "common.cuh"
 #include "internal.h"
 
 namespace fbb {
 
 constexpr int kDiffStages = 3;
-constexpr int kDiffPart = 16 * 128 + 16 * 2;  // floats of 16 rows of a share and map: the outputs, then {maximum, sum} of each row
+constexpr int kDiffPart = 16 * 128 + 16 * 2;  // floats of 16 rows of a part and map: the outputs, then {maximum, sum} of each row
 
 struct DiffSmem {
     static constexpr int kQOff = 0;                       // Q_1 | Q_2
     static constexpr int kStageOff = 2 * kTileBytes;      // stages of K_1 | K_2 | V columns 0..63 | V columns 64..127
     static constexpr int kStageBytes = 4 * kTileBytes;
-    static constexpr int kBarOff = kStageOff + kDiffStages * kStageBytes;
-    // q_full, w_ready, k_full[2][S], k_empty[2][S], v_full[S], v_empty[S], then of each map and half s_full, p_ready, pv_done
-    static constexpr int kNumBars = 2 + 6 * kDiffStages + 12;
-    static constexpr int kWeightOff = kBarOff + kNumBars * 8 + 16;  // [128] fp32
-    static constexpr int kBytes = kWeightOff + 128 * 4;
+    static constexpr int kRowOff = kStageOff + kDiffStages * kStageBytes;  // [2][128] row sums of the maps, [2][128] sums of squares of the halves
+    static constexpr int kWeightOff = kRowOff + 4 * 128 * 4;               // [128] fp32
+    static constexpr int kBarOff = kWeightOff + 128 * 4;
+    // q_full, q_empty, w_ready, o_free, k_full[2][S], k_empty[2][S], v_full[S], v_empty[S], then of each map and half s_full, p_ready, pv_done,
+    // then where the two maps' softmax warps of the same rows meet
+    static constexpr int kNumBars = 4 + 6 * kDiffStages + 12 + 8;
+    static constexpr int kBytes = kBarOff + kNumBars * 8 + 16;
 };
 static_assert(DiffSmem::kBytes <= 232448, "more shared memory than a CTA can have");
 
@@ -52,7 +56,8 @@ struct DiffArgs {
     float eps, out_scale, scale_log2;
     const int* lengths;      // keys of each batch entry, null: Nk
     int B, H, group;         // group = query heads per key head
-    int Nq, Nk, q_tiles, splits;
+    int Nq, Nk, q_tiles;
+    int splits, items;       // items = tiles x splits
     float* part;             // [tile][split][map][16-row group][kDiffPart], null when splits == 1
     int row_groups;          // of a tile that hold rows: min(8, ceil(Nq / 16))
 };
@@ -68,6 +73,70 @@ __device__ __forceinline__ void diff_share(int keys, int split, int splits, int&
         kb1 = (int)((unsigned)blocks * (unsigned)(split + 1) / (unsigned)splits);
     }
 }
+// A CTA's items: one of every gridDim.x, from the front and from the back of each such row in turn, so that the sums come out even
+// where the tiles' lengths fall along the row: batch entries are taken by falling number of keys (up to 32 of them, whose numbers the
+// lanes of a warp hold; more are taken in their order). All lanes of a warp go through the items together.
+struct DiffItems {
+    int w, round;         // item, and the row of gridDim.x items it is in
+    int b, h, qt;         // (b: the place until the lengths are known)
+    int keys, kb0, here;  // keys of the batch entry; first block and number of keys of the item
+    int order;            // the batch entry that is `lane`-th, and its keys times 32
+    __device__ __forceinline__ explicit DiffItems(const DiffArgs& a) {
+        w = (int)blockIdx.x;
+        round = 0;
+        decode(a);
+    }
+    __device__ __forceinline__ static bool sorted(const DiffArgs& a) { return a.lengths != nullptr && a.B <= 32 && a.Nk < (1 << 26); }
+    __device__ __forceinline__ void decode(const DiffArgs& a) {
+        const unsigned tile = a.splits > 1 ? (unsigned)w / (unsigned)a.splits : (unsigned)w;
+        const unsigned bh = tile / (unsigned)a.q_tiles;
+        qt = (int)(tile - bh * (unsigned)a.q_tiles);
+        b = a.B > 1 ? (int)(bh / (unsigned)a.H) : 0;
+        h = (int)bh - b * a.H;
+    }
+    // The rest of the set-up, which reads the lengths.
+    __device__ __forceinline__ void begin(const DiffArgs& a, int lane) {
+        if (sorted(a)) {
+            const int mine = lane < a.B ? diff_keys(a, lane) : 0;
+            int place = 0;
+            for (int j = 0; j < a.B; ++j) {
+                const int other = __shfl_sync(0xffffffffu, mine, j);
+                place += other > mine || (other == mine && j < lane);
+            }
+            for (int j = 0; j < a.B; ++j) {
+                const int entry = __shfl_sync(0xffffffffu, mine, j) * 32 + j;
+                if (__shfl_sync(0xffffffffu, place, j) == lane) order = entry;
+            }
+        }
+        item(a);
+    }
+    __device__ __forceinline__ void item(const DiffArgs& a) {
+        if (a.lengths == nullptr) {
+            keys = a.Nk;
+        } else if (sorted(a)) {
+            const int entry = __shfl_sync(0xffffffffu, order, b);
+            b = entry & 31;
+            keys = entry >> 5;
+        } else {
+            keys = w < a.items ? diff_keys(a, b) : 0;
+        }
+        int kb1;
+        diff_share(keys, a.splits > 1 ? (int)((unsigned)w % (unsigned)a.splits) : 0, a.splits, kb0, kb1);
+        here = min(keys, kb1 * FK) - kb0 * FK;
+    }
+    // Where the rows of a split go in the workspace: by the tile itself, not by its place.
+    __device__ __forceinline__ int64_t part(const DiffArgs& a) const {
+        return (((int64_t)b * a.H + h) * a.q_tiles + qt) * a.splits + (int)((unsigned)w % (unsigned)a.splits);
+    }
+    __device__ __forceinline__ bool more(const DiffArgs& a) const { return w < a.items; }
+    __device__ __forceinline__ void next(const DiffArgs& a) {
+        const int in_row = (int)((++round & 1) ? gridDim.x - 1u - blockIdx.x : blockIdx.x);
+        w = round * (int)gridDim.x + in_row;
+        if (w >= a.items) return;
+        decode(a);
+        item(a);
+    }
+};
 __device__ __forceinline__ float diff_weight(const DiffArgs& a, int col) {
     return a.weight_f32 ? reinterpret_cast<const float*>(a.weight)[col] : __half2float(reinterpret_cast<const __half*>(a.weight)[col]);
 }
@@ -108,6 +177,22 @@ __device__ __forceinline__ float4 ld_shared_f4(uint32_t addr) {
 
 constexpr int kDiffEarly = 2;  // key groups of eight exponentiated ahead of the vote on the running maximum (see kEarly in flash64.cu)
 
+// Four 32-bit values of each of the four lanes of a quad, [lane][k] -> [k][lane].
+__device__ __forceinline__ void quad_transpose(uint32_t* m, int cq) {
+#pragma unroll
+    for (int k = 0; k < 4; k += 2) {
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, (cq & 1) ? m[k] : m[k + 1], 1);
+        if (cq & 1) m[k] = got;
+        else m[k + 1] = got;
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, (cq & 2) ? m[k] : m[k + 2], 2);
+        if (cq & 2) m[k] = got;
+        else m[k + 2] = got;
+    }
+}
+
 __global__ void __launch_bounds__(640, 1)
 diff64_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
               const DiffArgs a) {
@@ -115,14 +200,16 @@ diff64_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     const uint32_t base = smem_u32(smem_raw);
     const uint32_t bar0 = base + S::kBarOff;
-    const uint32_t q_full = bar0, w_ready = bar0 + 8u;
-    auto k_full = [&](int t, int s) { return bar0 + 8u * (2 + t * kDiffStages + s); };
-    auto k_empty = [&](int t, int s) { return bar0 + 8u * (2 + (2 + t) * kDiffStages + s); };
-    auto v_full = [&](int s) { return bar0 + 8u * (2 + 4 * kDiffStages + s); };
-    auto v_empty = [&](int s) { return bar0 + 8u * (2 + 5 * kDiffStages + s); };
-    auto s_full = [&](int t, int half) { return bar0 + 8u * (2 + 6 * kDiffStages + 2 * t + half); };
-    auto p_ready = [&](int t, int half) { return bar0 + 8u * (2 + 6 * kDiffStages + 4 + 2 * t + half); };
-    auto pv_done = [&](int t, int half) { return bar0 + 8u * (2 + 6 * kDiffStages + 8 + 2 * t + half); };
+    const uint32_t q_full = bar0, q_empty = bar0 + 8u, w_ready = bar0 + 16u, o_free = bar0 + 24u;
+    constexpr int kK = 4, kV = kK + 4 * kDiffStages, kS = kV + 2 * kDiffStages;
+    auto k_full = [&](int t, int s) { return bar0 + 8u * (kK + t * kDiffStages + s); };
+    auto k_empty = [&](int t, int s) { return bar0 + 8u * (kK + (2 + t) * kDiffStages + s); };
+    auto v_full = [&](int s) { return bar0 + 8u * (kV + s); };
+    auto v_empty = [&](int s) { return bar0 + 8u * (kV + kDiffStages + s); };
+    auto s_full = [&](int t, int half) { return bar0 + 8u * (kS + 2 * t + half); };
+    auto p_ready = [&](int t, int half) { return bar0 + 8u * (kS + 4 + 2 * t + half); };
+    auto pv_done = [&](int t, int half) { return bar0 + 8u * (kS + 8 + 2 * t + half); };
+    auto meeting = [&](int u) { return bar0 + 8u * (kS + 12 + u); };
     volatile uint32_t* s_tmem = reinterpret_cast<volatile uint32_t*>(smem_raw + S::kBarOff + S::kNumBars * 8);
     volatile int* s_abort = reinterpret_cast<volatile int*>(smem_raw + S::kBarOff + S::kNumBars * 8 + 4);
 
@@ -130,9 +217,12 @@ diff64_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
     const int lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < S::kNumBars; ++i) {
-            // v_empty: both maps' issuers; p_ready: the eight softmax warps of a map
-            const int v0 = 2 + 5 * kDiffStages, p0 = 2 + 6 * kDiffStages + 4;
-            mbar_init(bar0 + 8u * i, i >= v0 && i < v0 + kDiffStages ? 2 : (i >= p0 && i < p0 + 4 ? 8 : 1));
+            int count = 1;
+            if (i == 1 || (i >= kV + kDiffStages && i < kS)) count = 2;  // q_empty, v_empty: both maps' issuers
+            if (i >= kS + 12) count = 2;
+            if (i == 3) count = 16;                                    // o_free: the softmax warps
+            if (i >= kS + 4 && i < kS + 8) count = 8;                  // p_ready: a map's softmax warps
+            mbar_init(bar0 + 8u * i, count);
         }
         *s_abort = 0;
         fence_barrier_init();
@@ -145,100 +235,116 @@ diff64_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
         tmem_alloc<512>(smem_u32(const_cast<uint32_t*>(s_tmem)));
         tmem_relinquish();
     }
-    const unsigned tile = a.splits > 1 ? blockIdx.x / (unsigned)a.splits : blockIdx.x;
-    const int split = (int)(blockIdx.x - tile * (unsigned)a.splits);
-    const int bh = (int)(tile / (unsigned)a.q_tiles), q0 = (int)(tile - (unsigned)bh * (unsigned)a.q_tiles) * FQ;
-    const int b = (int)((unsigned)bh / (unsigned)a.H), h = bh - b * a.H;
+    DiffItems it(a);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *s_tmem;
     grid_dependency_wait();
     grid_launch_dependents();
+    it.begin(a, lane);
 
-    const int keys = diff_keys(a, b);
-    int kb0, kb1;
-    diff_share(keys, split, a.splits, kb0, kb1);
-    const int here = min(keys - kb0 * FK, (kb1 - kb0) * FK);  // keys of this share, the last ones' block may be ragged
-    const int halves = (here + 63) / 64;                     // half-blocks that hold a key
-
-    if (warp == 0) {
-        if (lane == 0 && halves > 0) {
-            const int hk = a.group > 1 ? (int)((unsigned)h / (unsigned)a.group) : h;
-            mbar_arrive_expect_tx(q_full, 2 * kTileBytes);
-            for (int t = 0; t < 2; ++t) tma_load_4d(base + S::kQOff + t * kTileBytes, &tmap_q, q_full, 0, 2 * h + t, q0, b);
-            int s = 0;
+    if (warp < 4) {
+        setmaxnreg_dec<kRegsCtl>();
+        if (warp == 0) {
+            int s = 0, nq = 0;
             uint32_t ph = 0;
             bool ok = true;
 #pragma unroll 1
-            for (int kb = kb0; kb < kb1 && ok; ++kb) {
-                const uint32_t st = base + S::kStageOff + s * S::kStageBytes;
+            for (; it.more(a) && ok; it.next(a)) {
+                if (it.here <= 0) continue;
+                if (lane == 0) {
+                    const int b = it.b, h = it.h, hk = a.group > 1 ? (int)((unsigned)h / (unsigned)a.group) : h;
+                    ok = nq == 0 || mbar_wait(q_empty, (uint32_t)(nq - 1) & 1u, s_abort, DEV_TIMEOUT_SMEM_EMPTY, 32);
+                    if (ok) {
+                        mbar_arrive_expect_tx(q_full, 2 * kTileBytes);
+                        for (int t = 0; t < 2; ++t) tma_load_4d(base + S::kQOff + t * kTileBytes, &tmap_q, q_full, 0, 2 * h + t, it.qt * FQ, b);
+                    }
+                    const int kb1 = it.kb0 + (it.here + FK - 1) / FK;
 #pragma unroll 1
-                for (int t = 0; t < 2; ++t) {
-                    ok = ok && mbar_wait(k_empty(t, s), ph ^ 1u, s_abort, DEV_TIMEOUT_SMEM_EMPTY, 2 * s + t);
-                    if (!ok) break;
-                    mbar_arrive_expect_tx(k_full(t, s), kTileBytes);
-                    tma_load_4d(st + t * kTileBytes, &tmap_k, k_full(t, s), 0, 2 * hk + t, kb * FK, b);
+                    for (int kb = it.kb0; kb < kb1 && ok; ++kb) {
+                        const uint32_t st = base + S::kStageOff + s * S::kStageBytes;
+#pragma unroll 1
+                        for (int t = 0; t < 2; ++t) {
+                            ok = ok && mbar_wait(k_empty(t, s), ph ^ 1u, s_abort, DEV_TIMEOUT_SMEM_EMPTY, 2 * s + t);
+                            if (!ok) break;
+                            mbar_arrive_expect_tx(k_full(t, s), kTileBytes);
+                            tma_load_4d(st + t * kTileBytes, &tmap_k, k_full(t, s), 0, 2 * hk + t, kb * FK, b);
+                        }
+                        ok = ok && mbar_wait(v_empty(s), ph ^ 1u, s_abort, DEV_TIMEOUT_SMEM_EMPTY, 16 + s);
+                        if (!ok) break;
+                        mbar_arrive_expect_tx(v_full(s), 2 * kTileBytes);
+                        for (int t = 0; t < 2; ++t) tma_load_4d(st + (2 + t) * kTileBytes, &tmap_v, v_full(s), 64 * t, hk, kb * FK, b);
+                        if (++s == kDiffStages) { s = 0; ph ^= 1u; }
+                    }
                 }
-                ok = ok && mbar_wait(v_empty(s), ph ^ 1u, s_abort, DEV_TIMEOUT_SMEM_EMPTY, 16 + s);
-                if (!ok) break;
-                mbar_arrive_expect_tx(v_full(s), 2 * kTileBytes);
-                for (int t = 0; t < 2; ++t) tma_load_4d(st + (2 + t) * kTileBytes, &tmap_v, v_full(s), 64 * t, hk, kb * FK, b);
-                if (++s == kDiffStages) { s = 0; ph ^= 1u; }
+                ++nq;
+                ok = __all_sync(0xffffffffu, ok) != 0;
             }
             if (!ok) __nanosleep(20000);
-        }
-    } else if (warp < 3) {
-        const int t = warp - 1;
-        const uint32_t idesc_qk = make_idesc_f16(FQ, 64, true, false, false);
-        const uint32_t idesc_pv = make_idesc_f16(FQ, 128, true, false, true);
-        const uint64_t qd = smem_desc(base + S::kQOff + t * kTileBytes, make_smem_desc_hi(16, 1024));
-        const uint64_t kd0 = smem_desc(base + S::kStageOff + t * kTileBytes, make_smem_desc_hi(16, 1024));
-        const uint64_t vd0 = smem_desc(base + S::kStageOff + 2 * kTileBytes, make_smem_desc_hi(kTileBytes, 1024));  // column halves a tile apart
-        const uint32_t dS = tmem_base + t * 128, dO = tmem_base + 256 + t * 128;
-        auto all_ok = [&](bool mine) { return __all_sync(0xffffffffu, mine) != 0; };
-        // unit g: half g & 1 of block g / 2; 64 keys are 8 KB further in a tile of K or V
-        int ks = 0, vs = 0;  // stages of the next unit's K and V
-        uint32_t kph = 0, vph = 0;
-        auto scores = [&](int g) -> bool {
-            const int half = g & 1;
-            if (half == 0 && !all_ok(mbar_wait(k_full(t, ks), kph, s_abort, DEV_TIMEOUT_TMA_FULL, 2 * ks + t))) return false;
-            tc_fence_after();
-            const uint64_t kd = kd0 + (uint64_t)((ks * S::kStageBytes + half * (kTileBytes / 2)) >> 4);
-            umma_kblock_commit_warp(dS + 64u * half, qd, kd, idesc_qk, 0u, s_full(t, half));
-            if (half == 1) {
-                umma_commit_warp(k_empty(t, ks));
-                if (++ks == kDiffStages) { ks = 0; kph ^= 1u; }
-            }
-            return true;
-        };
-        bool ok = halves > 0 && all_ok(mbar_wait(q_full, 0, s_abort, DEV_TIMEOUT_TMA_FULL, 100));
-        ok = ok && scores(0);
-        if (ok && halves > 1) ok = scores(1);
+        } else if (warp < 3) {
+            const int t = warp - 1;
+            const uint32_t idesc_qk = make_idesc_f16(FQ, 64, true, false, false);
+            const uint32_t idesc_pv = make_idesc_f16(FQ, 128, true, false, true);
+            const uint64_t qd = smem_desc(base + S::kQOff + t * kTileBytes, make_smem_desc_hi(16, 1024));
+            const uint64_t kd0 = smem_desc(base + S::kStageOff + t * kTileBytes, make_smem_desc_hi(16, 1024));
+            const uint64_t vd0 = smem_desc(base + S::kStageOff + 2 * kTileBytes, make_smem_desc_hi(kTileBytes, 1024));  // column halves a tile apart
+            const uint32_t dS = tmem_base + t * 128, dO = tmem_base + 256 + t * 128;
+            auto all_ok = [&](bool mine) { return __all_sync(0xffffffffu, mine) != 0; };
+            // Units (half-blocks) are counted over all items, g, which gives the half of tensor memory and the barriers' phases, and inside
+            // an item, i: half i & 1 of a block, whose 64 keys are 8 KB further in a tile of K or V.
+            int ks = 0, vs = 0;  // stages of the next unit's K and V
+            uint32_t kph = 0, vph = 0;
+            auto scores = [&](uint32_t g, int i, bool last) -> bool {
+                if ((i & 1) == 0 && !all_ok(mbar_wait(k_full(t, ks), kph, s_abort, DEV_TIMEOUT_TMA_FULL, 2 * ks + t))) return false;
+                tc_fence_after();
+                const uint64_t kd = kd0 + (uint64_t)((ks * S::kStageBytes + (i & 1) * (kTileBytes / 2)) >> 4);
+                umma_kblock_commit_warp(dS + 64u * (g & 1u), qd, kd, idesc_qk, 0u, s_full(t, g & 1u));
+                if ((i & 1) == 1 || last) {
+                    umma_commit_warp(k_empty(t, ks));
+                    if (++ks == kDiffStages) { ks = 0; kph ^= 1u; }
+                }
+                if (last) umma_commit_warp(q_empty);
+                return true;
+            };
+            uint32_t g = 0;
+            int n = 0, nq = 0;  // items, and those with keys
+            bool ok = true;
 #pragma unroll 1
-        for (int g = 0; g < halves && ok; ++g) {
-            const int half = g & 1;
-            if (half == 0 && !all_ok(mbar_wait(v_full(vs), vph, s_abort, DEV_TIMEOUT_TMA_FULL, 16 + vs))) break;
-            const uint32_t vt = S::kStageOff + vs * S::kStageBytes + 2 * kTileBytes + half * (kTileBytes / 2);
-            if (g + 1 == halves && here < 64 * halves && kb0 * FK + here < a.Nk) {
-                // rows of V beyond the entry's keys hold whatever the tensor holds there (beyond the tensor the copy wrote zeros); both
-                // issuers write the same zeros
-                for (int i = (here - 64 * g) * 8 + lane; i < 64 * 8; i += 32)
-                    for (int c = 0; c < 2; ++c) st_shared_16(base + vt + c * kTileBytes + 16u * i, 0.f, 0.f, 0.f, 0.f);
-                fence_proxy_async_smem();
-                __syncwarp();
+            for (; it.more(a) && ok; it.next(a), ++n) {
+                const int here = it.here, halves = (here + 63) / 64;
+                if (here > 0) {
+                    ok = all_ok(mbar_wait(q_full, (uint32_t)nq & 1u, s_abort, DEV_TIMEOUT_TMA_FULL, 100));
+                    ++nq;
+                    ok = ok && scores(g, 0, halves == 1);
+                    if (ok && halves > 1) ok = scores(g + 1u, 1, halves == 2);
+                }
+                // the softmax warps have read the last item's O (every item's phase is waited for: none may be skipped)
+                if (ok && n > 0) ok = all_ok(mbar_wait(o_free, (uint32_t)(n - 1) & 1u, s_abort, DEV_TIMEOUT_TMEM_EMPTY, 40 + t));
+#pragma unroll 1
+                for (int i = 0; i < halves && ok; ++i, ++g) {
+                    if ((i & 1) == 0 && !all_ok(mbar_wait(v_full(vs), vph, s_abort, DEV_TIMEOUT_TMA_FULL, 16 + vs))) { ok = false; break; }
+                    const uint32_t vt = vs * S::kStageBytes + (i & 1) * (kTileBytes / 2);
+                    if (i + 1 == halves && here < 64 * halves && it.keys < a.Nk) {
+                        // rows of V beyond the entry's keys hold whatever the tensor holds there (beyond the tensor the copy wrote zeros);
+                        // both issuers write the same zeros
+                        const uint32_t at = base + S::kStageOff + 2 * kTileBytes + vt;
+                        for (int j = (here - 64 * i) * 8 + lane; j < 64 * 8; j += 32)
+                            for (int c = 0; c < 2; ++c) st_shared_16(at + c * kTileBytes + 16u * j, 0.f, 0.f, 0.f, 0.f);
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                    }
+                    if (!all_ok(mbar_wait(p_ready(t, g & 1u), (g >> 1) & 1u, s_abort, DEV_TIMEOUT_OTHER, 200 + 2 * t + (g & 1u)))) { ok = false; break; }
+                    tc_fence_after();
+                    umma_ts4_commit_warp(dO, dS + 64u * (g & 1u), vd0 + (uint64_t)(vt >> 4), idesc_pv, i > 0 ? 1u : 0u, pv_done(t, g & 1u));
+                    if ((i & 1) == 1 || i + 1 == halves) {
+                        umma_commit_warp(v_empty(vs));
+                        if (++vs == kDiffStages) { vs = 0; vph ^= 1u; }
+                    }
+                    if (i + 2 < halves) ok = scores(g + 2u, i + 2, i + 3 == halves);
+                }
             }
-            if (!all_ok(mbar_wait(p_ready(t, half), (g >> 1) & 1u, s_abort, DEV_TIMEOUT_OTHER, 200 + 2 * t + half))) break;
-            tc_fence_after();
-            umma_ts4_commit_warp(dO, dS + 64u * half, vd0 + (uint64_t)((vt - S::kStageOff - 2 * kTileBytes) >> 4), idesc_pv, g > 0 ? 1u : 0u, pv_done(t, half));
-            if (half == 1) {
-                umma_commit_warp(v_empty(vs));
-                if (++vs == kDiffStages) { vs = 0; vph ^= 1u; }
-            }
-            if (g + 2 < halves) ok = scores(g + 2);
-        }
-    } else if (warp == 3) {
-        if (a.weight != nullptr) {
+        } else if (a.weight != nullptr) {
             float* s_w = reinterpret_cast<float*>(smem_raw + S::kWeightOff);
 #pragma unroll
             for (int i = 0; i < 4; ++i) s_w[lane + 32 * i] = diff_weight(a, lane + 32 * i) * a.out_scale;
@@ -246,38 +352,61 @@ diff64_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
             if (lane == 0) mbar_arrive(w_ready);
         }
     } else {
+        setmaxnreg_inc<kRegsSoftmax>();
         const int u = (warp - 4) & 7;
         const int t = (warp - 4) >> 3;
         const int lane_base = (u & 3) * 32 + (u >> 2) * 16;
         const int cq = lane & 3;
-        const uint32_t tS = tmem_base + ((uint32_t)lane_base << 16) + t * 128;
-        const uint32_t tO = tmem_base + ((uint32_t)lane_base << 16) + 256 + t * 128;
+        const uint32_t tl = tmem_base + ((uint32_t)lane_base << 16);  // this warp's lanes
+        const uint32_t tS = tl + t * 128, tO = tl + 256 + t * 128;
         const float sl = a.scale_log2;
         const float lazy = kLazyMax / sl;
-        const int rowA = q0 + lane_base + (lane >> 2), rowB = rowA + 8;
-        if (q0 + lane_base >= a.Nq) {
-            // a warp of rows beyond Nq only keeps the barriers moving: S_t of unit g exists only after the issuer has taken P_t of unit g - 2
+        bool ok = true;
+        uint32_t g = 0;
+        int n = 0;
+        // Both maps' warps of these rows have got here (a barrier with a limit: a warp that gave up does not come).
+        uint32_t met = 0;
+        auto meet = [&]() {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(meeting(u));
+            ok = mbar_wait(meeting(u), met & 1u, s_abort, DEV_TIMEOUT_OTHER, 230 + u) && ok;
+            ++met;
+        };
+        // an item's end: O has been read (an earlier item's phase must be complete before this one's arrivals begin)
+        auto release = [&]() {
+            tc_fence_before();
+            ok = (n == 0 || mbar_wait(o_free, (uint32_t)(n - 1) & 1u, s_abort, DEV_TIMEOUT_OTHER, 44)) && ok;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(o_free);
+        };
 #pragma unroll 1
-            for (int g = 0; g < halves; ++g) {
-                if (!mbar_wait(s_full(t, g & 1), (g >> 1) & 1u, s_abort, DEV_TIMEOUT_TMEM_FULL, 2 * t + (g & 1))) break;
-                tc_fence_after();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(p_ready(t, g & 1));
+        for (; it.more(a) && ok; it.next(a), ++n) {
+            const int here = it.here, halves = (here + 63) / 64;
+            const int row0 = it.qt * FQ + lane_base, rowA = row0 + (lane >> 2), rowB = rowA + 8;
+            if (row0 >= a.Nq) {
+                // a warp of rows beyond Nq only keeps the barriers moving: S_t of unit g exists only after the issuer has taken P_t of unit g - 2
+#pragma unroll 1
+                for (int i = 0; i < halves && ok; ++i, ++g) {
+                    ok = mbar_wait(s_full(t, g & 1u), (g >> 1) & 1u, s_abort, DEV_TIMEOUT_TMEM_FULL, 2 * t + (g & 1u));
+                    tc_fence_after();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (ok && lane == 0) mbar_arrive(p_ready(t, g & 1u));
+                }
+                release();
+                continue;
             }
-        } else {
-            float fA = 1.f, fB = 1.f;  // factors of the map's rows in the result
-            if (t == 1 && a.splits == 1) {
-                fA = rowA < a.Nq ? a.lam[b * a.l_sb + rowA * a.l_sn + h * a.l_sh] : 0.f;
-                fB = rowB < a.Nq ? a.lam[b * a.l_sb + rowB * a.l_sn + h * a.l_sh] : 0.f;
+            const bool whole = a.splits == 1;
+            float lamA = 0.f, lamB = 0.f;
+            if (whole) {
+                const float* lam = a.lam + it.b * a.l_sb + it.h * a.l_sh;
+                if (rowA < a.Nq) lamA = lam[rowA * a.l_sn];
+                if (rowB < a.Nq) lamB = lam[rowB * a.l_sn];
             }
             float tA = 0.f, tB = 0.f;
             float mA = -INFINITY, mB = -INFINITY, lA = 0.f, lB = 0.f;
-            bool ok = true;
-            // one half-block; `last`: the one that may have keys beyond the entry's
-            auto unit = [&](int g, auto last) -> bool {
-                const int half = g & 1;
-                const uint32_t tSh = tS + 64u * half;
+            auto unit = [&](int i) -> bool {  // one half-block
+                const uint32_t half = g & 1u, tSh = tS + 64u * half;
                 if (!mbar_wait(s_full(t, half), (g >> 1) & 1u, s_abort, DEV_TIMEOUT_TMEM_FULL, 2 * t + half)) return false;
                 tc_fence_after();
                 uint32_t sc[32], pk[16];
@@ -285,19 +414,19 @@ diff64_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
                 tmem_ld_16x256b_x8(tSh, sc);
                 tmem_wait_ld();
                 tmem_tie32(sc);
-                if constexpr (decltype(last)::value) mask_frag(sc, 64 * g + 2 * cq, here);
+                if (64 * (i + 1) > here) mask_frag(sc, 64 * i + 2 * cq, here);  // (the last one may have keys beyond the entry's)
                 max_frag<8>(sc, mxA, mxB);
                 float2 accA = make_float2(0.f, 0.f), accB = make_float2(0.f, 0.f);
                 exp_frag<kDiffEarly>(sc, sl, mA, mB, accA, accB, pk);
-                if (g == 0 || __any_sync(0xffffffffu, mxA > tA || mxB > tB)) {
+                if (i == 0 || __any_sync(0xffffffffu, mxA > tA || mxB > tB)) {
                     mxA = fmaxf(mxA, __shfl_xor_sync(0xffffffffu, mxA, 1));
                     mxB = fmaxf(mxB, __shfl_xor_sync(0xffffffffu, mxB, 1));
                     mxA = fmaxf(mxA, __shfl_xor_sync(0xffffffffu, mxA, 2));
                     mxB = fmaxf(mxB, __shfl_xor_sync(0xffffffffu, mxB, 2));
                     const float nA = fmaxf(mA, mxA * sl), nB = fmaxf(mB, mxB * sl);
-                    if (g > 0) {
+                    if (i > 0) {
                         // the unit before this one may still be adding to O_t
-                        if (!mbar_wait(pv_done(t, half ^ 1), ((g - 1) >> 1) & 1u, s_abort, DEV_TIMEOUT_TMEM_FULL, 8 + 2 * t + half)) return false;
+                        if (!mbar_wait(pv_done(t, half ^ 1u), ((g - 1u) >> 1) & 1u, s_abort, DEV_TIMEOUT_TMEM_FULL, 8 + 2 * t + half)) return false;
                         tc_fence_after();
                         const float cA = ex2_approx(mA - nA), cB = ex2_approx(mB - nB);
 #pragma unroll 1
@@ -319,8 +448,8 @@ diff64_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
                     }
                     mA = nA;
                     mB = nB;
-                    tA = g == 0 ? mxA + lazy : fmaxf(tA, mxA + lazy);
-                    tB = g == 0 ? mxB + lazy : fmaxf(tB, mxB + lazy);
+                    tA = i == 0 ? mxA + lazy : fmaxf(tA, mxA + lazy);
+                    tB = i == 0 ? mxB + lazy : fmaxf(tB, mxB + lazy);
                     accA = accB = make_float2(0.f, 0.f);
                     exp_frag<kDiffEarly>(sc, sl, mA, mB, accA, accB, pk);
                 }
@@ -334,25 +463,19 @@ diff64_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
                 lB += accB.x + accB.y;
                 return true;
             };
-            const int plain = here / 64;  // halves full of keys
 #pragma unroll 1
-            for (int g = 0; g < plain && ok; ++g) ok = unit(g, std::false_type());
-            if (ok && plain < halves) ok = unit(plain, std::true_type());
-            if (ok && halves > 0) {
-                const int g = halves - 1;
-                ok = mbar_wait(pv_done(t, g & 1), (g >> 1) & 1u, s_abort, DEV_TIMEOUT_TMEM_FULL, 12 + t);
-            }
-            tc_fence_after();
+            for (int i = 0; i < halves && ok; ++i, ++g) ok = unit(i);
+            if (ok && halves > 0) ok = mbar_wait(pv_done(t, (g - 1u) & 1u), ((g - 1u) >> 1) & 1u, s_abort, DEV_TIMEOUT_TMEM_FULL, 12 + t);
             // a row's sum is spread over the four threads that share it
             lA += __shfl_xor_sync(0xffffffffu, lA, 1);
             lB += __shfl_xor_sync(0xffffffffu, lB, 1);
             lA += __shfl_xor_sync(0xffffffffu, lA, 2);
             lB += __shfl_xor_sync(0xffffffffu, lB, 2);
-            // What follows runs once: rolled loops over 16 columns at a time, because instructions that run once cost their fetch.
-            if (a.splits > 1) {
-                // the rows of this share for diff64_join_kernel (which asks for no share without keys)
+            tc_fence_after();
+            if (!whole) {
+                // a split's rows, for diff64_join_kernel (which asks for no split without keys)
                 if (halves > 0) {
-                    float* dst = a.part + (((int64_t)blockIdx.x * 2 + t) * a.row_groups + (lane_base >> 4)) * kDiffPart;
+                    float* dst = a.part + ((it.part(a) * 2 + t) * a.row_groups + (lane_base >> 4)) * kDiffPart;
                     float2* outA = reinterpret_cast<float2*>(dst + (lane >> 2) * 128 + 2 * cq);
 #pragma unroll 1
                     for (int c = 0; c < 8; ++c) {
@@ -362,82 +485,84 @@ diff64_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
                             outA[8 * c + 4 * i] = make_float2(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]));
-                            outA[8 * c + 4 * i + 8 * 64] = make_float2(__uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));  // row B
+                            if (rowB < a.Nq) outA[8 * c + 4 * i + 8 * 64] = make_float2(__uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
                         }
                     }
                     float2* stat = reinterpret_cast<float2*>(dst + 16 * 128);
                     if (cq == 0) stat[lane >> 2] = make_float2(mA, lA);
                     if (cq == 1) stat[(lane >> 2) + 8] = make_float2(mB, lB);
                 }
-            } else {
-                // Map 1's warps leave lam O_2 / l_2 in shared memory, where their twins of map 0, which hold the same elements of O_1, take it:
-                // 16 values of every thread in Q_2 and in each stage's K_2, which only map 1's products read (they have completed).
-                fA = halves > 0 ? fA / lA : 0.f;
-                fB = halves > 0 ? fB / lB : 0.f;
-                auto twin = [&](int c) {  // two 16-byte vectors, 4 KB apart, of columns 16 c ..
-                    const int quarter = c >> 1;
-                    return (quarter == 0 ? base + S::kQOff + kTileBytes : base + S::kStageOff + (quarter - 1) * S::kStageBytes + kTileBytes) +
-                           (uint32_t)((c & 1) * 8192 + (u * 32 + lane) * 16);
-                };
-                float sA = 0.f, sB = 0.f;
-                if (t == 0) named_bar_sync(1 + u, 64);
-#pragma unroll 1
-                for (int c = 0; c < 8; ++c) {
-                    uint32_t r[8];
-                    float o[8];
-                    tmem_ld_16x256b_x2(tO + 16u * c, r);
+                release();
+                continue;
+            }
+            // Columns 64 t .. 64 t + 63 of the tile's rows: o = O_1 / l_1 - lam O_2 / l_2. The other map's warp of these rows has waited for
+            // its last product when it arrives with its sums.
+            float* s_l = reinterpret_cast<float*>(smem_raw + S::kRowOff);
+            float* s_q = s_l + 256;
+            const int rA = lane_base + (lane >> 2);
+            float o[32];
+            if (halves > 0) {
+                if (cq == 0) {
+                    s_l[t * 128 + rA] = lA;
+                    s_l[t * 128 + rA + 8] = lB;
+                }
+                tc_fence_before();
+                meet();
+                tc_fence_after();
+                const float f1A = 1.f / s_l[rA], f1B = 1.f / s_l[rA + 8], f2A = lamA / s_l[128 + rA], f2B = lamB / s_l[128 + rA + 8];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t x[8], y[8];
+                    tmem_ld_16x256b_x2(tl + 256 + 64 * t + 16 * c, x);
+                    tmem_ld_16x256b_x2(tl + 384 + 64 * t + 16 * c, y);
                     tmem_wait_ld();
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) o[i] = halves > 0 ? __uint_as_float(r[i]) * ((i & 2) ? fB : fA) : 0.f;
-                    const uint32_t at = twin(c);
-                    if (t == 0) {
-                        const float4 x = ld_shared_f4(at), y = ld_shared_f4(at + 4096u);
-                        o[0] -= x.x, o[1] -= x.y, o[2] -= x.z, o[3] -= x.w, o[4] -= y.x, o[5] -= y.y, o[6] -= y.z, o[7] -= y.w;
+                    for (int i = 0; i < 8; ++i) o[8 * c + i] = __uint_as_float(x[i]) * ((i & 2) ? f1B : f1A) - __uint_as_float(y[i]) * ((i & 2) ? f2B : f2A);
+                }
+            } else {
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            if (i & 2) sB = fmaf(o[i], o[i], sB);
-                            else sA = fmaf(o[i], o[i], sA);
-                        }
-                    }
-                    st_shared_16(at, o[0], o[1], o[2], o[3]);
-                    st_shared_16(at + 4096u, o[4], o[5], o[6], o[7]);
+                for (int i = 0; i < 32; ++i) o[i] = 0.f;
+            }
+            release();
+            float scA = a.out_scale, scB = a.out_scale;
+            const bool norm = a.weight != nullptr && halves > 0;
+            if (norm) {
+                float sA = 0.f, sB = 0.f;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    if (i & 2) sB = fmaf(o[i], o[i], sB);
+                    else sA = fmaf(o[i], o[i], sA);
                 }
-                if (t == 1) named_bar_sync(1 + u, 64);
-                if (t == 0) {
-                    float rA = a.out_scale, rB = a.out_scale;
-                    const bool norm = a.weight != nullptr;
-                    if (norm) {
-                        sA += __shfl_xor_sync(0xffffffffu, sA, 1);
-                        sB += __shfl_xor_sync(0xffffffffu, sB, 1);
-                        sA += __shfl_xor_sync(0xffffffffu, sA, 2);
-                        sB += __shfl_xor_sync(0xffffffffu, sB, 2);
-                        rA = rsqrtf(sA * (1.f / 128.f) + a.eps);  // (the weight in shared memory holds out_scale)
-                        rB = rsqrtf(sB * (1.f / 128.f) + a.eps);
-                        ok = mbar_wait(w_ready, 0, s_abort, DEV_TIMEOUT_OTHER, 220) && ok;
-                    }
-                    // The warp's 16 rows of 256 bytes go through 4 KB of shared memory that only map 0's products read (Q_1, the first
-                    // stage's K_1), 16-byte units swizzled by the row, and leave by 16-byte stores, a row's by 16 lanes.
-                    const uint32_t st = (u < 4 ? base + S::kQOff : base + S::kStageOff) + (uint32_t)(u & 3) * 4096u;
-                    const uint32_t strow = (uint32_t)(lane & 15);
-                    const float* s_w = reinterpret_cast<const float*>(smem_raw + S::kWeightOff) + 2 * cq;
-#pragma unroll 1
-                    for (int c = 0; c < 8; ++c) {
-                        const float4 x = ld_shared_f4(twin(c)), y = ld_shared_f4(twin(c) + 4096u);
-                        const float2 one = make_float2(1.f, 1.f);
-                        const float2 w0 = norm ? *reinterpret_cast<const float2*>(s_w + 16 * c) : one, w1 = norm ? *reinterpret_cast<const float2*>(s_w + 16 * c + 8) : one;
-                        const uint32_t unit = (uint32_t)(2 * c + (lane >> 4)) ^ (strow & 7u);
-                        stmatrix_x4(st + strow * 256u + unit * 16u, pack_h2(x.x * rA * w0.x, x.y * rA * w0.y), pack_h2(x.z * rB * w0.x, x.w * rB * w0.y),
-                                    pack_h2(y.x * rA * w1.x, y.y * rA * w1.y), pack_h2(y.z * rB * w1.x, y.w * rB * w1.y));
-                    }
-                    __syncwarp();
-                    __half* dst = a.o + (int64_t)b * a.o_sb + (int64_t)h * a.o_sh + 8 * (lane & 15);
-#pragma unroll 2
-                    for (int i = 0; i < 8; ++i) {
-                        const int r = 2 * i + (lane >> 4), row = q0 + lane_base + r;
-                        const uint4 v = ld_shared_16(st + (uint32_t)r * 256u + (uint32_t)(((lane & 15) ^ (r & 7)) * 16));
-                        if (ok && row < a.Nq) *reinterpret_cast<uint4*>(dst + (int64_t)row * a.o_sn) = v;
-                    }
+                sA += __shfl_xor_sync(0xffffffffu, sA, 1);
+                sB += __shfl_xor_sync(0xffffffffu, sB, 1);
+                sA += __shfl_xor_sync(0xffffffffu, sA, 2);
+                sB += __shfl_xor_sync(0xffffffffu, sB, 2);
+                if (cq == 0) {
+                    s_q[t * 128 + rA] = sA;
+                    s_q[t * 128 + rA + 8] = sB;
                 }
+                ok = mbar_wait(w_ready, 0, s_abort, DEV_TIMEOUT_OTHER, 220) && ok;
+                meet();
+                scA = rsqrtf((s_q[rA] + s_q[128 + rA]) * (1.f / 128.f) + a.eps);  // (the weight in shared memory holds out_scale)
+                scB = rsqrtf((s_q[rA + 8] + s_q[128 + rA + 8]) * (1.f / 128.f) + a.eps);
+            }
+            const float* s_w = reinterpret_cast<const float*>(smem_raw + S::kWeightOff) + 64 * t + 2 * cq;
+            __half* out = a.o + (int64_t)it.b * a.o_sb + (int64_t)it.h * a.o_sh + 64 * t + 8 * cq;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                // a quad's lanes hold two columns each of four groups of eight: afterwards each holds the eight of one
+                uint32_t hA[4], hB[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float* v = o + 16 * j + 4 * k;
+                    const float2 w = norm ? *reinterpret_cast<const float2*>(s_w + 32 * j + 8 * k) : make_float2(1.f, 1.f);
+                    hA[k] = pack_h2(v[0] * scA * w.x, v[1] * scA * w.y);
+                    hB[k] = pack_h2(v[2] * scB * w.x, v[3] * scB * w.y);
+                }
+                quad_transpose(hA, cq);
+                quad_transpose(hB, cq);
+                if (ok && rowA < a.Nq) *reinterpret_cast<uint4*>(out + (int64_t)rowA * a.o_sn + 32 * j) = make_uint4(hA[0], hA[1], hA[2], hA[3]);
+                if (ok && rowB < a.Nq) *reinterpret_cast<uint4*>(out + (int64_t)rowB * a.o_sn + 32 * j) = make_uint4(hB[0], hB[1], hB[2], hB[3]);
             }
         }
     }
@@ -581,14 +706,14 @@ int launch_diff64(const void* q, const void* k, const void* v, void* o, int B, i
     a.B = B, a.H = H, a.group = H / Hk;
     a.Nq = Nq, a.Nk = Nk, a.q_tiles = (Nq + FQ - 1) / FQ;
     a.splits = diff64_splits(B, Nq, Nk, H);
+    const int64_t items = (int64_t)B * H * a.q_tiles * a.splits;
+    if (items > 0x3FFFFFFFll) return fail(FBB_ERR_SHAPE, "diff64: too many query tiles (%lld)", (long long)items);
+    a.items = (int)items;
     a.row_groups = diff64_row_groups(Nq);
     const int64_t need = diff64_workspace_bytes(B, Nq, Nk, H);
     if (need > 0 && (ws == nullptr || ws_bytes < need))
         return fail(FBB_ERR_SHAPE, "diff64: workspace of %lld bytes, %lld needed", (long long)(ws != nullptr ? ws_bytes : 0), (long long)need);
     a.part = need > 0 ? reinterpret_cast<float*>(ws) : nullptr;
-    const int64_t ctas = (int64_t)B * H * a.q_tiles * a.splits;
-    if (ctas > 0x7FFFFFFFll) return fail(FBB_ERR_SHAPE, "diff64: too many query tiles (%lld)", (long long)ctas);
-
     CUtensorMap tq, tk, tv;
     struct { CUtensorMap* map; const void* p; const int64_t* st; uint64_t cols, heads, rows; } t[3] = {
         {&tq, q, qs, 64, 2 * (uint64_t)H, (uint64_t)Nq}, {&tk, k, ks, 64, 2 * (uint64_t)Hk, (uint64_t)Nk}, {&tv, v, vs, 128, (uint64_t)Hk, (uint64_t)Nk}};
@@ -609,7 +734,7 @@ int launch_diff64(const void* q, const void* k, const void* v, void* o, int B, i
         if (e != cudaSuccess) return fail((int)e, "cudaFuncSetAttribute(diff64_kernel): %s", cudaGetErrorString(e));
         if (dev >= 0 && dev < 64) configured[dev] = true;
     }
-    cudaError_t e = launch_pdl(diff64_kernel, dim3((unsigned)ctas), dim3(640), DiffSmem::kBytes, stream, tq, tk, tv, a);
+    cudaError_t e = launch_pdl(diff64_kernel, dim3((unsigned)(a.items < num_sms() ? a.items : num_sms())), dim3(640), DiffSmem::kBytes, stream, tq, tk, tv, a);
     if (e != cudaSuccess) return fail((int)e, "diff64_kernel launch: %s", cudaGetErrorString(e));
     if (a.splits > 1) {
         e = launch_pdl(diff64_join_kernel, dim3((unsigned)(B * (int64_t)H * a.q_tiles * a.row_groups)), dim3(512), 0, stream, a);
