@@ -16,63 +16,38 @@
 namespace fbb {
 
 struct AdapterArgs {
+    Requests requests;
+    const float* scale;   // [L]
+    int M, N, K, r;
+    // blocks form
+    int tile_rows;        // of the linear kernel
+    int pass_cols, stages;  // columns of h in a pass, a multiple of 16 up to kDownCols; tiles of x on their way
+    __half* h;
+    // rows form
     const __half* x;
     int64_t ldx;
     const __half* down;   // [L, r, K]
-    const float* scale;   // [L]
-    const int* ids;       // [S]
-    const int* offsets;   // [S + 1] or null: `each` rows a request
-    int M, N, K, L, r, S, each;
-    // blocks form
-    int tile_rows;
-    __half* h;
-    int4* tiles;
-    int* list;
-    // rows form
     const __half* up;     // [L, N, r]
     float* delta;
     int cols;
 };
 
-__device__ __forceinline__ int adapter_begin(const AdapterArgs& a, int s) {
-    return a.offsets != nullptr ? min(max(__ldcg(a.offsets + s), 0), a.M) : s * a.each;
-}
-__device__ __forceinline__ int adapter_id(const AdapterArgs& a, int s) {
-    const int id = __ldcg(a.ids + s);
-    return id >= 0 && id < a.L ? id : -1;
-}
-// First request whose end lies beyond `row` (S if none), by the whole warp: 32 probes a round.
-__device__ __forceinline__ int adapter_request(const AdapterArgs& a, int row, int lane) {
-    if (a.offsets == nullptr) return min(row / a.each, a.S);
-    int lo = 0, hi = a.S;
-    while (lo < hi) {
-        const int step = (hi - lo + 31) / 32, probe = min(lo + (lane + 1) * step - 1, hi - 1);
-        const uint32_t beyond = __ballot_sync(0xffffffffu, adapter_begin(a, probe + 1) > row);
-        if (beyond == 0u) return hi;
-        const int first = __ffs(beyond) - 1;
-        hi = min(lo + (first + 1) * step - 1, hi - 1);  // its probe: the answer is there or before it, behind the probe ahead
-        lo += first * step;
-        if (step == 1) return hi;
-    }
-    return lo;
-}
-
 // h of the blocks form: a CTA takes 128 rows of x and multiplies them with the first matrices of their requests, up to 64 columns of
-// h at a time (several requests side by side where the rank leaves room), as UMMAs of 128 x 64 fed by TMA: x is read once for most tiles,
-// and the launch is bound by that. x's tiles start ahead of the look-up of the requests, which is a chain of dependent loads. The
-// first CTA of a row tile also writes the tables that the linear kernel goes by.
+// h at a time, or 128 where tiles hold many requests (several requests side by side where the rank leaves room), as UMMAs fed by TMA: x is
+// read once for most tiles. Many tiles are bound by that read (180 MB at 21920 x 4096: 28 us), few by latency: x's tiles start ahead of
+// the look-up of the requests, which is a chain of dependent loads, and as many are on their way as shared memory holds.
 //   warp 0   look-up of the requests, then TMA producer      warp 1   UMMA issuer      warps 2..5   rows of h out of tensor memory
-constexpr int kDownCols = 64;     // of h in a pass
-constexpr int kDownStages = 4;
+constexpr int kDownCols = 128;
+constexpr int kDownMaxStages = 12;
 constexpr int kDownMaxRequests = 128;
 constexpr int kDownThreads = 192;
-struct DownSmem {
+struct DownSmem {  // ring of {x [128 x 64], first matrices [pass_cols x 64]} | barriers | table of requests
     static constexpr int kABytes = BM * BK * 2;
-    static constexpr int kStageBytes = kABytes + kDownCols * BK * 2;
-    static constexpr int kBarOff = kDownStages * kStageBytes;
-    static constexpr int kNumBars = 2 * kDownStages + 4;  // full, empty, accumulator full[2], empty[2]
-    static constexpr int kTableOff = kBarOff + kNumBars * 8 + 16;
-    static constexpr int kDynamic = 1024 + kTableOff + (int)(kDownMaxRequests * sizeof(int4)) + 16;
+    static constexpr int kNumBars = 2 * kDownMaxStages + 4;  // full, empty, accumulator full[2], empty[2]
+    static constexpr int kTailBytes = kNumBars * 8 + 16 + (int)(kDownMaxRequests * sizeof(int4)) + 16;
+    static int stage_bytes(int pass_cols) { return kABytes + pass_cols * BK * 2; }
+    static int dynamic_bytes(int pass_cols, int stages) { return 1024 + stages * stage_bytes(pass_cols) + kTailBytes; }
+    static constexpr int kMaxDynamic = 227 * 1024;
 };
 
 __global__ void __launch_bounds__(kDownThreads) adapter_down_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_down,
@@ -80,21 +55,22 @@ __global__ void __launch_bounds__(kDownThreads) adapter_down_kernel(const __grid
     using S = DownSmem;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
-    uint8_t* gen = smem_raw + (base - raw);
-    const uint32_t bar0 = base + S::kBarOff;
+    const uint32_t stage_bytes = (uint32_t)(S::kABytes + a.pass_cols * BK * 2), ring = (uint32_t)a.stages * stage_bytes;
+    uint8_t* tail = smem_raw + (base - raw) + ring;
+    const uint32_t bar0 = base + ring;
     auto full_bar = [&](int s) { return bar0 + 8u * s; };
-    auto empty_bar = [&](int s) { return bar0 + 8u * (kDownStages + s); };
-    auto tfull_bar = [&](int i) { return bar0 + 8u * (2 * kDownStages + i); };
-    auto tempty_bar = [&](int i) { return bar0 + 8u * (2 * kDownStages + 2 + i); };
-    volatile uint32_t* s_tmem = reinterpret_cast<volatile uint32_t*>(gen + S::kBarOff + S::kNumBars * 8);
-    volatile int* s_abort = reinterpret_cast<volatile int*>(gen + S::kBarOff + S::kNumBars * 8 + 4);
-    int4* s_req = reinterpret_cast<int4*>(gen + S::kTableOff);  // {request, first row, one behind its last, adapter}
+    auto empty_bar = [&](int s) { return bar0 + 8u * (kDownMaxStages + s); };
+    auto tfull_bar = [&](int i) { return bar0 + 8u * (2 * kDownMaxStages + i); };
+    auto tempty_bar = [&](int i) { return bar0 + 8u * (2 * kDownMaxStages + 2 + i); };
+    volatile uint32_t* s_tmem = reinterpret_cast<volatile uint32_t*>(tail + S::kNumBars * 8);
+    volatile int* s_abort = reinterpret_cast<volatile int*>(tail + S::kNumBars * 8 + 4);
+    int4* s_req = reinterpret_cast<int4*>(tail + S::kNumBars * 8 + 16);  // {request, first row, one behind its last, adapter}
     volatile int* s_count = reinterpret_cast<volatile int*>(s_req + kDownMaxRequests);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int num_kb = (a.K + BK - 1) / BK;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kDownStages; ++s) {
+        for (int s = 0; s < a.stages; ++s) {
             mbar_init(full_bar(s), 2);  // x's bytes, the adapters' bytes
             mbar_init(empty_bar(s), 1);
         }
@@ -121,25 +97,24 @@ __global__ void __launch_bounds__(kDownThreads) adapter_down_kernel(const __grid
 
     const int m0 = (int)blockIdx.x * BM, m1 = min(m0 + BM, a.M);
     const int tile = m0 / a.tile_rows, t0 = tile * a.tile_rows, t1 = min(t0 + a.tile_rows, a.M);
-    const int ahead = min(num_kb, kDownStages);
+    const int ahead = min(num_kb, a.stages);
     if (warp == 0) {
         if (lane == 0) {
             for (int s = 0; s < ahead; ++s) {
                 mbar_arrive_expect_tx(full_bar(s), S::kABytes);
-                tma_load_2d(base + s * S::kStageBytes, &tmap_x, full_bar(s), s * BK, m0);
+                tma_load_2d(base + s * stage_bytes, &tmap_x, full_bar(s), s * BK, m0);
             }
         }
         __syncwarp();
-        const int first = adapter_request(a, t0, lane), end = min(adapter_request(a, t1 - 1, lane) + 1, a.S);
-        int count = 0, here = 0;
+        int first, end, here = 0;
+        a.requests.of_rows(t0, t1, lane, first, end);
         for (int s0 = first; s0 < end; s0 += 32) {
             const int s = s0 + lane;
             int id = -1, b = 0, e = 0;
             if (s < end) {
-                b = adapter_begin(a, s);
-                e = adapter_begin(a, s + 1);
-                if (max(b, t0) < min(e, t1)) id = adapter_id(a, s);
-                if (m0 == t0) a.list[tile + s] = id;
+                b = a.requests.begin(s);
+                e = a.requests.begin(s + 1);
+                id = a.requests.adapter_in(s, t0, t1);
             }
             const uint32_t any = __ballot_sync(0xffffffffu, id >= 0), mine = __ballot_sync(0xffffffffu, id >= 0 && max(b, m0) < min(e, m1));
             const int at = here + __popc(mine & ((1u << lane) - 1u));
@@ -149,93 +124,78 @@ __global__ void __launch_bounds__(kDownThreads) adapter_down_kernel(const __grid
                 uint4* dst = reinterpret_cast<uint4*>(a.h + ((int64_t)(tile + s0 + __ffs(rest) - 1) * a.tile_rows + (m0 - t0)) * a.r);
                 for (int i = lane; i < BM * (a.r >> 3); i += 32) dst[i] = make_uint4(0u, 0u, 0u, 0u);
             }
-            count += __popc(any);
             here += __popc(mine);
         }
-        if (lane == 0) {
-            *s_count = min(here, kDownMaxRequests);
-            if (m0 == t0) a.tiles[tile] = make_int4(first, end, count, 0);
-        }
+        if (lane == 0) *s_count = min(here, kDownMaxRequests);
     }
     __syncthreads();
-    // Passes: columns [c0, c0 + cols) of the requests' r columns each, side by side; a rank above 64 takes two passes a request.
-    const int requests = *s_count, per_pass = a.r >= kDownCols ? 1 : kDownCols / a.r;
-    const int halves = a.r > kDownCols ? 2 : 1, passes = (requests + per_pass - 1) / per_pass * halves;
-    auto pass_at = [&](int p, int& req0, int& n, int& c0, int& cols) {
-        req0 = p / halves * per_pass;
-        n = min(per_pass, requests - req0);
-        c0 = (p % halves) * kDownCols;
-        cols = min(kDownCols, a.r - c0);
-    };
+    const int requests = *s_count, per_pass = a.pass_cols / a.r, passes = (requests + per_pass - 1) / per_pass;  // per_pass requests side by side
     if (warp == 0) {
-        if (lane == 0) {
-            int s = 0;
-            uint32_t ph = 0;
-            bool ok = true;
-            for (int p = 0; p < passes && ok; ++p) {
-                int req0, n, c0, cols;
-                pass_at(p, req0, n, c0, cols);
-                for (int kb = 0; kb < num_kb; ++kb) {
-                    const uint32_t st = base + s * S::kStageBytes;
-                    if (p > 0 || kb >= ahead) {
-                        if (!mbar_wait(empty_bar(s), ph ^ 1u, s_abort, DEV_TIMEOUT_SMEM_EMPTY, s)) { ok = false; break; }
-                        mbar_arrive_expect_tx(full_bar(s), S::kABytes);
-                        tma_load_2d(st, &tmap_x, full_bar(s), kb * BK, m0);
-                    }
-                    // boxes of min(64, r) rows, which may reach into the next adapter's: they land behind this request's, or nowhere that is read
-                    mbar_arrive_expect_tx(full_bar(s), (uint32_t)(n * min(kDownCols, a.r) * BK * 2));
-                    for (int i = 0; i < n; ++i)
-                        tma_load_2d(st + S::kABytes + (uint32_t)(i * cols * BK * 2), &tmap_down, full_bar(s), kb * BK, s_req[req0 + i].w * a.r + c0);
-                    if (++s == kDownStages) { s = 0; ph ^= 1u; }
+        // (the whole warp, one elected lane issues: see common.cuh)
+        int s = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        for (int p = 0; p < passes && ok; ++p) {
+            const int req0 = p * per_pass, n = min(per_pass, requests - req0);
+            const int row = s_req[req0 + min(lane, n - 1)].w * a.r;  // lane i: of request req0 + i (per_pass is 16 at most)
+            for (int kb = 0; kb < num_kb; ++kb) {
+                const uint32_t st = base + s * stage_bytes;
+                if (p > 0 || kb >= ahead) {
+                    if (__all_sync(0xffffffffu, mbar_wait(empty_bar(s), ph ^ 1u, s_abort, DEV_TIMEOUT_SMEM_EMPTY, s)) == 0) { ok = false; break; }
+                    if (lane == 0) mbar_arrive_expect_tx(full_bar(s), S::kABytes);
+                    __syncwarp();
+                    tma_load_2d_warp(st, &tmap_x, full_bar(s), kb * BK, m0);
                 }
+                if (lane == 0) mbar_arrive_expect_tx(full_bar(s), (uint32_t)(n * a.r * BK * 2));
+                __syncwarp();
+                for (int i = 0; i < n; ++i)
+                    tma_load_2d_warp(st + S::kABytes + (uint32_t)(i * a.r * BK * 2), &tmap_down, full_bar(s), kb * BK, __shfl_sync(0xffffffffu, row, i));
+                if (++s == a.stages) { s = 0; ph ^= 1u; }
             }
-            if (passes == 0)  // nobody waits for what was sent ahead, but it must land before the CTA leaves
-                for (int i = 0; i < ahead; ++i) {
-                    mbar_arrive(full_bar(i));
-                    ok = ok && mbar_wait(full_bar(i), 0, s_abort, DEV_TIMEOUT_TMA_FULL, i);
-                }
-            if (!ok) __nanosleep(20000);
         }
+        if (passes == 0)  // nobody waits for what was sent ahead, but it must land before the CTA leaves
+            for (int i = 0; i < ahead; ++i) {
+                if (lane == 0) mbar_arrive(full_bar(i));
+                __syncwarp();
+                ok = ok && mbar_wait(full_bar(i), 0, s_abort, DEV_TIMEOUT_TMA_FULL, i);
+            }
+        if (!ok) __nanosleep(20000);
     } else if (warp == 1) {
         constexpr uint64_t desc_hi = make_smem_desc_hi(16, 1024);
-        const uint64_t adesc0 = smem_desc(base, desc_hi);
         auto all_ok = [&](bool mine) { return __all_sync(0xffffffffu, mine) != 0; };
         int s = 0;
         uint32_t ph = 0;
         bool ok = true;
         for (int p = 0; p < passes && ok; ++p) {
-            int req0, n, c0, cols;
-            pass_at(p, req0, n, c0, cols);
-            const int acc = p & 1;
+            const int n = min(per_pass, requests - p * per_pass), acc = p & 1;
             ok = all_ok(mbar_wait(tempty_bar(acc), (((uint32_t)p >> 1) & 1u) ^ 1u, s_abort, DEV_TIMEOUT_TMEM_EMPTY, acc));
             if (!ok) break;
             tc_fence_after();
-            const uint32_t idesc = make_idesc_f16(BM, (n * cols + 15) / 16 * 16, true, false, false);
+            const uint32_t idesc = make_idesc_f16(BM, (n * a.r + 15) / 16 * 16, true, false, false);
             for (int kb = 0; kb < num_kb; ++kb) {
                 if (!all_ok(mbar_wait(full_bar(s), ph, s_abort, DEV_TIMEOUT_TMA_FULL, s))) { ok = false; break; }
                 tc_fence_after();
-                const uint64_t adesc = adesc0 + (uint64_t)(s * (S::kStageBytes >> 4));
+                const uint64_t adesc = smem_desc(base + s * stage_bytes, desc_hi);
                 umma_kblock_commit_warp(tmem_base + (uint32_t)(acc * kDownCols), adesc, adesc + (uint64_t)(S::kABytes >> 4), idesc, kb != 0 ? 1u : 0u, empty_bar(s));
-                if (++s == kDownStages) { s = 0; ph ^= 1u; }
+                if (++s == a.stages) { s = 0; ph ^= 1u; }
             }
             if (ok) umma_commit_warp(tfull_bar(acc));
         }
     } else {
         const int quad = warp & 3, row = m0 + quad * 32 + lane;
         for (int p = 0; p < passes; ++p) {
-            int req0, n, c0, cols;
-            pass_at(p, req0, n, c0, cols);
-            const int acc = p & 1;
+            const int req0 = p * per_pass, n = min(per_pass, requests - req0), acc = p & 1;
+            const float scales = __ldcg(a.scale + s_req[req0 + min(lane, n - 1)].w);  // lane i: of request req0 + i (per_pass is 16 at most)
             if (!mbar_wait(tfull_bar(acc), ((uint32_t)p >> 1) & 1u, s_abort, DEV_TIMEOUT_TMEM_FULL, acc)) break;
             tc_fence_after();
             for (int i = 0; i < n; ++i) {
                 const int4 req = s_req[req0 + i];
-                const float scale = row >= req.y && row < req.z ? __ldcg(a.scale + req.w) : 0.f;
+                const float scale = __shfl_sync(0xffffffffu, scales, i);
                 const bool mine = row >= req.y && row < req.z;
-                uint4* dst = reinterpret_cast<uint4*>(a.h + ((int64_t)(tile + req.x) * a.tile_rows + (row - t0)) * a.r + c0);
-                for (int c = 0; c < cols; c += 8) {
+                uint4* dst = reinterpret_cast<uint4*>(a.h + ((int64_t)(tile + req.x) * a.tile_rows + (row - t0)) * a.r);
+                for (int c = 0; c < a.r; c += 8) {
                     uint32_t v[8];
-                    tmem_ld8(tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * kDownCols + i * cols + c), v);
+                    tmem_ld8(tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * kDownCols + i * a.r + c), v);
                     tmem_wait_ld();
                     // rows of other requests are zeros, whatever their products are
                     dst[c >> 3] = mine ? make_uint4(pack_h2(__uint_as_float(v[0]) * scale, __uint_as_float(v[1]) * scale), pack_h2(__uint_as_float(v[2]) * scale, __uint_as_float(v[3]) * scale),
@@ -265,8 +225,8 @@ __global__ void __launch_bounds__(256) adapter_rows_kernel(const AdapterArgs a) 
     grid_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int m = (int)blockIdx.x, n0 = (int)blockIdx.y * a.cols, n1 = min(n0 + a.cols, a.N);
-    const int s = adapter_request(a, m, lane);
-    const int id = s < a.S && adapter_begin(a, s) <= m ? adapter_id(a, s) : -1;
+    const int s = a.requests.at_row(m, lane);
+    const int id = s < a.requests.S && a.requests.begin(s) <= m ? a.requests.adapter(s) : -1;
     float* delta = a.delta + (int64_t)m * a.N;
     if (id < 0) {
         for (int n = n0 + threadIdx.x; n < n1; n += 256) delta[n] = 0.f;
@@ -275,20 +235,28 @@ __global__ void __launch_bounds__(256) adapter_rows_kernel(const AdapterArgs a) 
     const uint4* x = reinterpret_cast<const uint4*>(a.x + (int64_t)m * a.ldx);
     const int vecs = a.K >> 3;
     const float scale = __ldcg(a.scale + id);
-    for (int n = warp; n < a.r; n += 8) {
+    // two products at a time: their loads wait for memory together
+    for (int n = 2 * warp; n < a.r; n += 16) {
         const uint4* d = reinterpret_cast<const uint4*>(a.down + ((int64_t)id * a.r + n) * a.K);
-        float2 acc = make_float2(0.f, 0.f);
+        float2 acc0 = make_float2(0.f, 0.f), acc1 = acc0;
 #pragma unroll 4
         for (int v = lane; v < vecs; v += 32) {
-            const uint4 xv = x[v], dv = __ldg(d + v);
-            const __half2 *xh = reinterpret_cast<const __half2*>(&xv), *dh = reinterpret_cast<const __half2*>(&dv);
+            const uint4 xv = x[v], d0 = __ldg(d + v), d1 = __ldg(d + vecs + v);
+            const __half2 *xh = reinterpret_cast<const __half2*>(&xv), *h0 = reinterpret_cast<const __half2*>(&d0), *h1 = reinterpret_cast<const __half2*>(&d1);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc = ffma2(__half22float2(xh[e]), __half22float2(dh[e]), acc);
+            for (int e = 0; e < 4; ++e) {
+                const float2 xf = __half22float2(xh[e]);
+                acc0 = ffma2(xf, __half22float2(h0[e]), acc0);
+                acc1 = ffma2(xf, __half22float2(h1[e]), acc1);
+            }
         }
-        float sum = acc.x + acc.y;
+        float sum0 = acc0.x + acc0.y, sum1 = acc1.x + acc1.y;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (lane == 0) s_h[n] = sum * scale;
+        for (int o = 16; o > 0; o >>= 1) {
+            sum0 += __shfl_xor_sync(0xffffffffu, sum0, o);
+            sum1 += __shfl_xor_sync(0xffffffffu, sum1, o);
+        }
+        if (lane == 0) s_h[n] = sum0 * scale, s_h[n + 1] = sum1 * scale;
     }
     __syncthreads();
     for (int n = n0 + threadIdx.x; n < n1; n += 256) {
@@ -324,51 +292,44 @@ static AdapterForm adapter_form(int64_t M, int N, int K, bool swiglu, int r, int
     const int n_out = swiglu ? N / 2 : N, sms = num_sms();
     AdapterForm f = {};
     auto tiles = [&](int rows, int bn) { return ((M + rows - 1) / rows) * (int64_t)((n_out + (swiglu ? bn / 2 : bn) - 1) / (swiglu ? bn / 2 : bn)); };
-    f.rows = M < 8 * (int64_t)S && M <= 512;
-    if (const char* e = getenv("FBB_ADAPTER_FORM")) f.rows = e[0] == 'r';  // rows | blocks: tuning and test aid
+    // What the forms add to the layer itself, us, fitted to measurements on B200 (rows / blocks, K = N = 1024, rank 16): 512 rows of 64
+    // requests 8.4 / 18, of 16 9 / 6.2; 2000 of 1000 19 / 58 (est.); 1200 of 75 (K = 768, N = 2304) 21.6 / 10.9. Rows: both matrices of every row's
+    // adapter are read once per row. Blocks: a product with either matrix per request and row tile.
+    const double rows_us = 4.3 + (double)M * r * ((double)K + N) * 2.0 / 6e6, per_tile = 1.0 + 128.0 * S / (double)M;
+    f.rows = M * (int64_t)N <= (1 << 26) && rows_us < 3.2 + per_tile * (0.4 + 0.03 * r);
     const int pairs = gemm_pairs_enabled() ? (swiglu ? max_pairs<256, true>() : max_pairs<256, false>()) : 0;
-    if (!f.rows && pairs > 0 && tiles(2 * BM, 256) > pairs / 2) {
-        f.bn = 256;
-        f.pairs = true;
-    } else {
-        f.bn = !swiglu && tiles(BM, 128) <= sms / 2 ? 64 : 128;
+    f.pairs = !f.rows && pairs > 0 && tiles(2 * BM, 256) > pairs / 2;
+    f.bn = f.pairs ? 256 : (!swiglu && tiles(BM, 128) <= sms / 2 ? 64 : 128);
+    if (const char* e = getenv("FBB_ADAPTER_FORM")) {  // r | s64 | s128 | p256: tuning and test aid
+        f.rows = e[0] == 'r';
+        f.pairs = e[0] == 'p' && pairs > 0;
+        f.bn = f.pairs ? 256 : (e[0] == 's' && e[1] == '6' && !swiglu ? 64 : 128);
     }
     return f;
 }
 
-// Workspace: h, the tile table and the list of the blocks form, each on a 256-byte boundary, or the rows form's delta.
-struct AdapterSpace {
-    int64_t tiles, list, bytes;
-};
-static AdapterSpace adapter_space(const AdapterForm& f, int64_t M, int N, int r, int S) {
-    AdapterSpace w = {};
-    auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
-    if (f.rows) {
-        w.bytes = up(M * N * (int64_t)sizeof(float));
-        return w;
-    }
+// Workspace: h, or the rows form's delta.
+static int64_t adapter_space(const AdapterForm& f, int64_t M, int N, int r, int S) {
     const int64_t tile_rows = f.pairs ? 2 * BM : BM, n_tiles = (M + tile_rows - 1) / tile_rows;
-    w.tiles = up((n_tiles + S) * tile_rows * r * 2);
-    w.list = w.tiles + up(n_tiles * (int64_t)sizeof(int4));
-    w.bytes = w.list + up((n_tiles + S) * (int64_t)sizeof(int));
-    return w;
+    return f.rows ? M * N * (int64_t)sizeof(float) : (n_tiles + S) * tile_rows * r * 2;
 }
 
 int64_t adapter_linear_workspace_bytes(int64_t M, int N, int K, int epilogue, int r, int S) {
     if (M <= 0 || S <= 0) return 0;
-    return adapter_space(adapter_form(M, N, K, epilogue == FBB_EPI_SWIGLU, r, S), M, N, r, S).bytes;
+    return adapter_space(adapter_form(M, N, K, epilogue == FBB_EPI_SWIGLU, r, S), M, N, r, S);
 }
 
 template <int BN, bool SWIGLU, bool CTA2, AdaptMode ADAPT>
 static int launch_adapter_variant(const CUtensorMap& ta, const CUtensorMap& tw, const CUtensorMap& th, const CUtensorMap& tu, const CUtensorMap& tc, GemmArgs g,
                                   const AdaptArgs& ad, cudaStream_t stream) {
     using S = GemmSmem<BN, CTA2>;
+    constexpr int kDynamic = S::kDynamic + 4 * S::kStages;  // and a number per stage
     auto kern = linear_adapter_kernel<BN, SWIGLU, CTA2, ADAPT>;
     static bool configured[64] = {};
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64 || !configured[dev]) {
-        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kDynamic);
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kDynamic);
         if (e != cudaSuccess) return fail((int)e, "cudaFuncSetAttribute(linear_adapter_kernel): %s", cudaGetErrorString(e));
         if (dev >= 0 && dev < 64) configured[dev] = true;
     }
@@ -379,7 +340,7 @@ static int launch_adapter_variant(const CUtensorMap& ta, const CUtensorMap& tw, 
     if (tiles > 0x7FFFFFFFll) return fail(FBB_ERR_SHAPE, "adapter_linear: too many tiles (%lld)", (long long)tiles);
     g.wide_tiles = (int)tiles;
     const int most = CTA2 ? max_pairs<BN, SWIGLU>() : num_sms(), workers = tiles < most ? (int)tiles : most;
-    const cudaError_t e = launch_pdl_cluster(kern, dim3((unsigned)(CTA2 ? 2 * workers : workers)), dim3(kGemmThreads), S::kDynamic, stream, CTA2 ? 2u : 1u, ta, tw, th,
+    const cudaError_t e = launch_pdl_cluster(kern, dim3((unsigned)(CTA2 ? 2 * workers : workers)), dim3(kGemmThreads), kDynamic, stream, CTA2 ? 2u : 1u, ta, tw, th,
                                              tu, tc, g, ad);
     if (e != cudaSuccess) return fail((int)e, "linear_adapter_kernel launch: %s", cudaGetErrorString(e));
     return FBB_OK;
@@ -390,26 +351,32 @@ int launch_adapter_linear(const void* A, const void* W, void* C, const void* bia
                           const int* offsets, int S, void* ws, int64_t ws_bytes, cudaStream_t stream) {
     const bool swiglu = epilogue == FBB_EPI_SWIGLU;
     const AdapterForm f = adapter_form(M, N, K, swiglu, r, S);
-    const AdapterSpace space = adapter_space(f, M, N, r, S);
-    if (ws == nullptr || ws_bytes < space.bytes)
-        return fail(FBB_ERR_SHAPE, "adapter_linear: workspace of %lld bytes, %lld needed", (long long)(ws != nullptr ? ws_bytes : 0), (long long)space.bytes);
-    uint8_t* w8 = reinterpret_cast<uint8_t*>(ws);
+    const int64_t need = adapter_space(f, M, N, r, S);
+    if (ws == nullptr || ws_bytes < need)
+        return fail(FBB_ERR_SHAPE, "adapter_linear: workspace of %lld bytes, %lld needed", (long long)(ws != nullptr ? ws_bytes : 0), (long long)need);
     const int tile_rows = f.pairs ? 2 * BM : BM;
     const int64_t h_rows = ((M + tile_rows - 1) / tile_rows + S) * tile_rows;
     if (h_rows > 0x7FFFFFFFll) return fail(FBB_ERR_SHAPE, "adapter_linear: too many requests (%d) for %lld rows", S, (long long)M);
 
     AdapterArgs d = {};
+    d.requests.ids = ids, d.requests.offsets = offsets;
+    d.requests.S = S, d.requests.each = offsets != nullptr ? 0 : (int)(M / S), d.requests.M = (int)M, d.requests.L = L;
+    d.scale = scale;
+    d.M = (int)M, d.N = N, d.K = K, d.r = r;
+    d.tile_rows = tile_rows;
+    d.h = reinterpret_cast<__half*>(ws);
     d.x = reinterpret_cast<const __half*>(A);
     d.ldx = lda;
     d.down = reinterpret_cast<const __half*>(down);
     d.up = reinterpret_cast<const __half*>(up);
-    d.scale = scale, d.ids = ids, d.offsets = offsets;
-    d.M = (int)M, d.N = N, d.K = K, d.L = L, d.r = r, d.S = S, d.each = offsets != nullptr ? 0 : (int)(M / S);
-    d.tile_rows = tile_rows;
-    d.h = reinterpret_cast<__half*>(ws);
-    d.tiles = reinterpret_cast<int4*>(w8 + space.tiles);
-    d.list = reinterpret_cast<int*>(w8 + space.list);
     d.delta = reinterpret_cast<float*>(ws);
+    // Columns of h in a pass: room for several requests where a tile has more than a couple. One CTA with all of shared memory where that
+    // gives every tile an SM, else two on each.
+    const int down_tiles = (int)((M + BM - 1) / BM);
+    d.pass_cols = M < 64 * (int64_t)S || r > 64 ? kDownCols : 64;
+    const int room = (down_tiles <= num_sms() ? DownSmem::kMaxDynamic : DownSmem::kMaxDynamic / 2 - 1024) - 1024 - DownSmem::kTailBytes;
+    d.stages = room / DownSmem::stage_bytes(d.pass_cols);
+    if (d.stages > kDownMaxStages) d.stages = kDownMaxStages;
 
     // boxes: 128 rows of A and h, 64 columns of h in the first launch; of W and the adapters' second matrices the rows that one CTA loads
     // per k-block
@@ -421,7 +388,7 @@ int launch_adapter_linear(const void* A, const void* W, void* C, const void* bia
         {&tc, C, (uint64_t)(swiglu ? N / 2 : N), (uint64_t)M, ldc, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B},
         {&th, ws, (uint64_t)r, (uint64_t)h_rows, r, BK, BM, CU_TENSOR_MAP_SWIZZLE_128B},
         {&tu, up, (uint64_t)r, (uint64_t)L * (uint64_t)N, r, BK, w_rows, CU_TENSOR_MAP_SWIZZLE_128B},
-        {&td, down, (uint64_t)K, (uint64_t)L * (uint64_t)r, K, BK, (uint32_t)(r < kDownCols ? r : kDownCols), CU_TENSOR_MAP_SWIZZLE_128B}};
+        {&td, down, (uint64_t)K, (uint64_t)L * (uint64_t)r, K, BK, (uint32_t)r, CU_TENSOR_MAP_SWIZZLE_128B}};
     for (int i = 0; i < (f.rows ? 3 : 6); ++i) {
         const uint64_t dims[2] = {maps[i].cols, maps[i].rows};
         const int64_t st[2] = {1, maps[i].stride};
@@ -442,11 +409,11 @@ int launch_adapter_linear(const void* A, const void* W, void* C, const void* bia
         int dev = 0;
         cudaGetDevice(&dev);
         if (dev < 0 || dev >= 64 || !configured[dev]) {
-            e = cudaFuncSetAttribute(adapter_down_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, DownSmem::kDynamic);
+            e = cudaFuncSetAttribute(adapter_down_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, DownSmem::kMaxDynamic);
             if (e != cudaSuccess) return fail((int)e, "cudaFuncSetAttribute(adapter_down_kernel): %s", cudaGetErrorString(e));
             if (dev >= 0 && dev < 64) configured[dev] = true;
         }
-        e = launch_pdl(adapter_down_kernel, dim3((unsigned)((M + BM - 1) / BM)), dim3(kDownThreads), DownSmem::kDynamic, stream, ta, td, d);
+        e = launch_pdl(adapter_down_kernel, dim3((unsigned)down_tiles), dim3(kDownThreads), (size_t)DownSmem::dynamic_bytes(d.pass_cols, d.stages), stream, ta, td, d);
     }
     if (e != cudaSuccess) return fail((int)e, "adapter kernel launch: %s", cudaGetErrorString(e));
 
@@ -461,8 +428,7 @@ int launch_adapter_linear(const void* A, const void* W, void* C, const void* bia
     g.act = epilogue == FBB_EPI_GELU ? 1 : 0;
     g.gemv_row0 = (int)M;
     AdaptArgs ad = {};
-    ad.tiles = d.tiles;
-    ad.list = d.list;
+    ad.requests = d.requests;
     ad.delta = d.delta;
     ad.r_blocks = (r + BK - 1) / BK;
 

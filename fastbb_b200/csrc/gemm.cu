@@ -124,10 +124,42 @@ __device__ __forceinline__ void remainder_rows_by_gemv(const GemmArgs& g, bool s
 
 // What a launch beside the shared projection adds (adapters.cu): of every row tile the products of its requests' adapters.
 enum AdaptMode { kAdaptNone, kAdaptBlocks, kAdaptRows };
+// Which rows are whose: request s has rows [offsets[s], offsets[s + 1]), or `each` rows, and adapter ids[s] (-1 or any id that is none: none).
+struct Requests {
+    const int* ids;      // [S]
+    const int* offsets;  // [S + 1] or null
+    int S, each, M, L;
+    __device__ __forceinline__ int begin(int s) const { return offsets != nullptr ? min(max(__ldcg(offsets + s), 0), M) : s * each; }
+    __device__ __forceinline__ int adapter(int s) const {
+        const int id = __ldcg(ids + s);
+        return id >= 0 && id < L ? id : -1;
+    }
+    // First request whose end lies beyond `row` (S if none), by the whole warp: 32 probes a round.
+    __device__ __forceinline__ int at_row(int row, int lane) const {
+        if (offsets == nullptr) return min((int)((unsigned)row / (unsigned)each), S);
+        int lo = 0, hi = S;
+        while (lo < hi) {
+            const int step = (hi - lo + 31) / 32, probe = min(lo + (lane + 1) * step - 1, hi - 1);
+            const uint32_t beyond = __ballot_sync(0xffffffffu, begin(probe + 1) > row);
+            if (beyond == 0u) return hi;
+            const int first = __ffs(beyond) - 1;
+            hi = min(lo + (first + 1) * step - 1, hi - 1);  // its probe: the answer is there or before it, behind the probe ahead
+            lo += first * step;
+            if (step == 1) return hi;
+        }
+        return lo;
+    }
+    // The requests of rows [r0, r1), by the whole warp: those from `first` up to `end`, of which some may have no row there or no adapter.
+    __device__ __forceinline__ void of_rows(int r0, int r1, int lane, int& first, int& end) const {
+        first = at_row(r0, lane);
+        end = min(at_row(r1 - 1, lane) + 1, S);
+    }
+    // Adapter of request s if it has one and rows among [r0, r1), else -1.
+    __device__ __forceinline__ int adapter_in(int s, int r0, int r1) const { return max(begin(s), r0) < min(begin(s + 1), r1) ? adapter(s) : -1; }
+};
 struct AdaptArgs {
+    Requests requests;
     // blocks
-    const int4* tiles;         // of each row tile {first request, one behind its last, products to add, 0}
-    const int* list;           // adapter of request s in tile t at t + s, -1: none
     const CUtensorMap* map_h;  // h of request s in tile t from row (t + s) * tile rows on, rows of other requests zero
     const CUtensorMap* map_up; // the adapters' second matrices [adapters * N, r]
     int r_blocks;              // 64-element k-blocks of the rank
@@ -158,6 +190,8 @@ __device__ __forceinline__ void linear_umma_body(const CUtensorMap& tmap_a, cons
     auto tempty_bar = [&](int a) { return bar0 + 8u * (2 * kStages + 2 + a); };
     volatile uint32_t* s_tmem = reinterpret_cast<volatile uint32_t*>(gen + S::kBarOffset + S::kNumBars * 8);
     volatile int* s_abort = reinterpret_cast<volatile int*>(gen + S::kBarOffset + S::kNumBars * 8 + 4);
+    // (adapters) of the stage with a tile's last k-block of x and W: how many more the tile has
+    volatile int* s_extra = reinterpret_cast<volatile int*>(gen + S::kBytes);
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
@@ -225,8 +259,11 @@ __device__ __forceinline__ void linear_umma_body(const CUtensorMap& tmap_a, cons
                 int m0, n0, w;
                 item_at(item, m0, n0, w);
                 const int nt = n0 / kOutCols;
-                for (int kb = 0; kb < num_kb; ++kb) {
-                    if (__all_sync(0xffffffffu, mbar_wait(empty_bar(s), ph ^ 1u, s_abort, DEV_TIMEOUT_SMEM_EMPTY, s)) == 0) { ok = false; break; }
+                // the requests of the tile's rows, the adapters of the first 32, and how many have one
+                const int tile = item / g.tiles_n, r0 = tile * kTileRows, r1 = min(r0 + kTileRows, g.M);
+                int first = 0, end = 0, slot0 = -1, extra = 0;
+                auto load = [&](int kb) -> bool {
+                    if (__all_sync(0xffffffffu, mbar_wait(empty_bar(s), ph ^ 1u, s_abort, DEV_TIMEOUT_SMEM_EMPTY, s)) == 0) return false;
                     const uint32_t sa = base + s * S::kStageBytes;
                     const uint32_t sb = sa + S::kABytes;
                     if constexpr (CTA2) {
@@ -244,14 +281,31 @@ __device__ __forceinline__ void linear_umma_body(const CUtensorMap& tmap_a, cons
                         if (SWIGLU) tma_load_2d_warp(sb + S::kBBytes / 2, &tmap_w, full_bar(s), kb * BK, g.N / 2 + nt * (BN / 2));
                     }
                     if (++s == kStages) { s = 0; ph ^= 1u; }
+                    return true;
+                };
+                // (with adapters the look-up of the requests runs, the ring full, ahead of the last k-block; as a condition inside the loop
+                // it cost 10 us of 170)
+                const int plain_kb = ADAPT == kAdaptBlocks ? num_kb - 1 : num_kb;
+                for (int kb = 0; kb < plain_kb; ++kb)
+                    if (!load(kb)) { ok = false; break; }
+                if constexpr (ADAPT == kAdaptBlocks) {
+                    if (!ok) break;
+                    ad.requests.of_rows(r0, r1, lane, first, end);
+                    for (int s0 = first; s0 < end; s0 += 32) {
+                        const int of = s0 + lane < end ? ad.requests.adapter_in(s0 + lane, r0, r1) : -1;
+                        if (s0 == first) slot0 = of;
+                        extra += __popc(__ballot_sync(0xffffffffu, of >= 0));
+                    }
+                    // (the stage is free: the issuer reads a stage's number before it multiplies what is in it)
+                    if (__all_sync(0xffffffffu, mbar_wait(empty_bar(s), ph ^ 1u, s_abort, DEV_TIMEOUT_SMEM_EMPTY, s)) == 0) { ok = false; break; }
+                    if (lane == 0) s_extra[s] = extra * ad.r_blocks;
+                    __syncwarp();
+                    ok = load(plain_kb);
                 }
                 if constexpr (ADAPT == kAdaptBlocks) {
                     // the adapters of the tile's requests: k-blocks of h (zero outside the request's rows) and of the adapter's second matrix
-                    grid_dependency_wait();
-                    const int tile = item / g.tiles_n;
-                    const int4 of = __ldcg(ad.tiles + tile);
-                    for (int s0 = of.x; s0 < of.y && ok; s0 += 32) {
-                        const int slot = s0 + lane < of.y ? __ldcg(ad.list + tile + s0 + lane) : -1;
+                    for (int s0 = first; s0 < end && ok; s0 += 32) {
+                        const int slot = s0 == first ? slot0 : (s0 + lane < end ? ad.requests.adapter_in(s0 + lane, r0, r1) : -1);
                         for (uint32_t todo = __ballot_sync(0xffffffffu, slot >= 0); todo != 0u && ok; todo &= todo - 1u) {
                             const int i = __ffs(todo) - 1;
                             const int up0 = __shfl_sync(0xffffffffu, slot, i) * g.N, h0 = (tile + s0 + i) * kTileRows + (int)rank * BM;
@@ -259,12 +313,21 @@ __device__ __forceinline__ void linear_umma_body(const CUtensorMap& tmap_a, cons
                                 if (__all_sync(0xffffffffu, mbar_wait(empty_bar(s), ph ^ 1u, s_abort, DEV_TIMEOUT_SMEM_EMPTY, s)) == 0) { ok = false; break; }
                                 const uint32_t sa = base + s * S::kStageBytes;
                                 const uint32_t sb = sa + S::kABytes;
+                                // the second matrix needs nothing of the kernel that makes h
                                 if constexpr (CTA2) {
                                     const int wrow = SWIGLU ? (rank == 0 ? nt * (BN / 2) : g.N / 2 + nt * (BN / 2)) : nt * BN + (int)rank * (BN / 2);
-                                    tma_load_2d_two_pair_warp(full_bar(s), rank == 0 ? 2u * S::kStageBytes : 0u, sa, ad.map_h, kb * BK, h0, sb, ad.map_up, kb * BK, up0 + wrow);
+                                    if (rank == 0 && lane == 0) mbar_arrive_expect_tx(full_bar(s), 2u * S::kStageBytes);
+                                    __syncwarp();
+                                    tma_load_2d_pair_warp(sb, ad.map_up, full_bar(s), kb * BK, up0 + wrow);
+                                    grid_dependency_wait();
+                                    tma_load_2d_pair_warp(sa, ad.map_h, full_bar(s), kb * BK, h0);
                                 } else {
-                                    tma_load_2d_two_warp(full_bar(s), S::kStageBytes, sa, ad.map_h, kb * BK, h0, sb, ad.map_up, kb * BK, up0 + (SWIGLU ? nt * (BN / 2) : nt * BN));
+                                    if (lane == 0) mbar_arrive_expect_tx(full_bar(s), S::kStageBytes);
+                                    __syncwarp();
+                                    tma_load_2d_warp(sb, ad.map_up, full_bar(s), kb * BK, up0 + (SWIGLU ? nt * (BN / 2) : nt * BN));
                                     if (SWIGLU) tma_load_2d_warp(sb + S::kBBytes / 2, ad.map_up, full_bar(s), kb * BK, up0 + g.N / 2 + nt * (BN / 2));
+                                    grid_dependency_wait();
+                                    tma_load_2d_warp(sa, ad.map_h, full_bar(s), kb * BK, h0);
                                 }
                                 if (++s == kStages) { s = 0; ph ^= 1u; }
                             }
@@ -293,9 +356,8 @@ __device__ __forceinline__ void linear_umma_body(const CUtensorMap& tmap_a, cons
             if (!all_ok(mbar_wait(tempty_bar(acc), acc_ph ^ 1u, s_abort, DEV_TIMEOUT_TMEM_EMPTY, acc))) break;
             tc_fence_after();
             const uint32_t d_tmem = tmem_base + (uint32_t)(acc * BN);
-            int total_kb = num_kb;
-            for (int kb = 0; kb < total_kb; ++kb) {
-                if (!all_ok(mbar_wait(full_bar(s), ph, s_abort, DEV_TIMEOUT_TMA_FULL, s))) { ok = false; break; }
+            auto multiply = [&](int kb) -> bool {
+                if (!all_ok(mbar_wait(full_bar(s), ph, s_abort, DEV_TIMEOUT_TMA_FULL, s))) return false;
                 tc_fence_after();
                 const uint64_t adesc = adesc0 + (uint64_t)(s * (S::kStageBytes >> 4));
                 const uint64_t bdesc = adesc + (uint64_t)(S::kABytes >> 4);
@@ -305,12 +367,18 @@ __device__ __forceinline__ void linear_umma_body(const CUtensorMap& tmap_a, cons
                     umma_kblock_commit_warp(d_tmem, adesc, bdesc, idesc, kb != 0 ? 1u : 0u, empty_bar(s));  // stage reusable once these UMMAs have read it
                 }
                 if (++s == kStages) { s = 0; ph ^= 1u; }
-                if constexpr (ADAPT == kAdaptBlocks) {
-                    if (kb + 1 == num_kb) {
-                        grid_dependency_wait();
-                        total_kb = num_kb + __ldcg(ad.tiles + item / g.tiles_n).z * ad.r_blocks;
-                    }
-                }
+                return true;
+            };
+            const int plain_kb = ADAPT == kAdaptBlocks ? num_kb - 1 : num_kb;
+            for (int kb = 0; kb < plain_kb; ++kb)
+                if (!multiply(kb)) { ok = false; break; }
+            if constexpr (ADAPT == kAdaptBlocks) {
+                // the last k-block of x and W, with which the producer says how many more there are
+                ok = ok && all_ok(mbar_wait(full_bar(s), ph, s_abort, DEV_TIMEOUT_TMA_FULL, s));
+                if (!ok) break;
+                const int extra = s_extra[s];
+                ok = multiply(plain_kb);
+                for (int kb = 0; kb < extra && ok; ++kb) ok = multiply(1);
             }
             if (!ok) break;
             if constexpr (CTA2) umma_commit_pair_warp(tfull_bar(acc));  // both CTAs' accumulators complete
