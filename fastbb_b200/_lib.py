@@ -32,7 +32,10 @@ _vp, _i32, _i64, _f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_
 
 def on(device):
     """Context manager that makes `device` current for the enclosed C calls (a no-op when it already is)."""
-    return torch.cuda.device(device) if device.index != torch.cuda.current_device() else contextlib.nullcontext()
+    return _HERE_ALREADY if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
+
+
+_HERE_ALREADY = contextlib.nullcontext()
 
 
 class BlockDesc(ctypes.Structure):

@@ -53,9 +53,13 @@ constexpr int kTmapSlots = 2048;
 TmapEntry g_tmap_cache[kTmapSlots];
 std::mutex g_tmap_mutex;
 uint64_t tmap_hash(const TmapKey& k) {
-    uint64_t h = 1469598103934665603ull;
-    const unsigned char* p = reinterpret_cast<const unsigned char*>(&k);
-    for (size_t i = 0; i < sizeof(TmapKey); ++i) h = (h ^ p[i]) * 1099511628211ull;
+    static_assert(sizeof(TmapKey) % sizeof(uint64_t) == 0, "hashed in words");
+    uint64_t words[sizeof(TmapKey) / sizeof(uint64_t)], h = 1469598103934665603ull;
+    memcpy(words, &k, sizeof(TmapKey));
+    for (uint64_t w : words) {
+        h = (h ^ w) * 1099511628211ull;
+        h ^= h >> 29;  // the slot is taken from the low bits, which a product of aligned addresses alone leaves alike
+    }
     return h;
 }
 }  // namespace
