@@ -4,9 +4,9 @@
 // Two launches: one makes h = scale (x A_a^T), rounded (in the blocks form) to fp16 because the tensor cores take it so (2^-11 of each value, as the
 // projection's own output is rounded), and the linear kernel adds h B_a^T to the accumulator it holds anyway. The second launch starts
 // under the first (its product with W needs nothing of it) and waits for it where it needs h. Two forms of the pair:
-//  blocks  h is laid out per (row tile t, request s in it) as block t + s of a tile's rows with zeros outside the request's (the
-//          requests of one tile follow one another, so t + s is a number of its own), and the linear kernel runs each as k-blocks behind
-//          those of x and W: one k-block of 64 per request and tile for ranks up to 64.
+//  blocks  h is [M, r], and the linear kernel runs it as k-blocks behind those of x and W: of every request in a row tile one k-block of 64
+//          (for ranks up to 64) against its adapter's second matrix, which adds to the request's rows of the accumulator alone (the
+//          lanes of tensor memory that a product leaves as they are are an operand of the instruction)
 //  rows    for few rows of many requests, where that would be a k-block per row or so: the first launch multiplies each row with both
 //          of its adapter's matrices on the CUDA cores (bound by reading those), and the linear kernel's epilogue adds that in fp32.
 // Rows of no request (ahead of offsets[0], behind offsets[S]) and of requests with an id out of [0, adapters) get x W^T alone.
@@ -20,7 +20,6 @@ struct AdapterArgs {
     const float* scale;   // [L]
     int M, N, K, r;
     // blocks form
-    int tile_rows;        // of the linear kernel
     int pass_cols, stages;  // columns of h in a pass, a multiple of 16 up to kDownCols; tiles of x on their way
     __half* h;
     // rows form
@@ -64,7 +63,7 @@ __global__ void __launch_bounds__(kDownThreads) adapter_down_kernel(const __grid
     auto tempty_bar = [&](int i) { return bar0 + 8u * (2 * kDownMaxStages + 2 + i); };
     volatile uint32_t* s_tmem = reinterpret_cast<volatile uint32_t*>(tail + S::kNumBars * 8);
     volatile int* s_abort = reinterpret_cast<volatile int*>(tail + S::kNumBars * 8 + 4);
-    int4* s_req = reinterpret_cast<int4*>(tail + S::kNumBars * 8 + 16);  // {request, first row, one behind its last, adapter}
+    int4* s_req = reinterpret_cast<int4*>(tail + S::kNumBars * 8 + 16);  // {first row, one behind its last, adapter, 0}
     volatile int* s_count = reinterpret_cast<volatile int*>(s_req + kDownMaxRequests);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -96,7 +95,6 @@ __global__ void __launch_bounds__(kDownThreads) adapter_down_kernel(const __grid
     grid_launch_dependents();
 
     const int m0 = (int)blockIdx.x * BM, m1 = min(m0 + BM, a.M);
-    const int tile = m0 / a.tile_rows, t0 = tile * a.tile_rows, t1 = min(t0 + a.tile_rows, a.M);
     const int ahead = min(num_kb, a.stages);
     if (warp == 0) {
         if (lane == 0) {
@@ -107,23 +105,12 @@ __global__ void __launch_bounds__(kDownThreads) adapter_down_kernel(const __grid
         }
         __syncwarp();
         int first, end, here = 0;
-        a.requests.of_rows(t0, t1, lane, first, end);
+        a.requests.of_rows(m0, m1, lane, first, end);
         for (int s0 = first; s0 < end; s0 += 32) {
-            const int s = s0 + lane;
-            int id = -1, b = 0, e = 0;
-            if (s < end) {
-                b = a.requests.begin(s);
-                e = a.requests.begin(s + 1);
-                id = a.requests.adapter_in(s, t0, t1);
-            }
-            const uint32_t any = __ballot_sync(0xffffffffu, id >= 0), mine = __ballot_sync(0xffffffffu, id >= 0 && max(b, m0) < min(e, m1));
+            const int s = s0 + lane, id = s < end ? a.requests.adapter_in(s, m0, m1) : -1;
+            const uint32_t mine = __ballot_sync(0xffffffffu, id >= 0);
             const int at = here + __popc(mine & ((1u << lane) - 1u));
-            if (((mine >> lane) & 1u) != 0u && at < kDownMaxRequests) s_req[at] = make_int4(s, b, e, id);
-            // of the tile's requests, those with no rows among this CTA's leave zeros here
-            for (uint32_t rest = any & ~mine; rest != 0u; rest &= rest - 1u) {
-                uint4* dst = reinterpret_cast<uint4*>(a.h + ((int64_t)(tile + s0 + __ffs(rest) - 1) * a.tile_rows + (m0 - t0)) * a.r);
-                for (int i = lane; i < BM * (a.r >> 3); i += 32) dst[i] = make_uint4(0u, 0u, 0u, 0u);
-            }
+            if (id >= 0 && at < kDownMaxRequests) s_req[at] = make_int4(a.requests.begin(s), a.requests.begin(s + 1), id, 0);
             here += __popc(mine);
         }
         if (lane == 0) *s_count = min(here, kDownMaxRequests);
@@ -137,7 +124,7 @@ __global__ void __launch_bounds__(kDownThreads) adapter_down_kernel(const __grid
         bool ok = true;
         for (int p = 0; p < passes && ok; ++p) {
             const int req0 = p * per_pass, n = min(per_pass, requests - req0);
-            const int row = s_req[req0 + min(lane, n - 1)].w * a.r;  // lane i: of request req0 + i (per_pass is 16 at most)
+            const int row = s_req[req0 + min(lane, n - 1)].z * a.r;  // lane i: of request req0 + i (per_pass is 16 at most)
             for (int kb = 0; kb < num_kb; ++kb) {
                 const uint32_t st = base + s * stage_bytes;
                 if (p > 0 || kb >= ahead) {
@@ -185,22 +172,21 @@ __global__ void __launch_bounds__(kDownThreads) adapter_down_kernel(const __grid
         const int quad = warp & 3, row = m0 + quad * 32 + lane;
         for (int p = 0; p < passes; ++p) {
             const int req0 = p * per_pass, n = min(per_pass, requests - req0), acc = p & 1;
-            const float scales = __ldcg(a.scale + s_req[req0 + min(lane, n - 1)].w);  // lane i: of request req0 + i (per_pass is 16 at most)
+            const float scales = __ldcg(a.scale + s_req[req0 + min(lane, n - 1)].z);  // lane i: of request req0 + i (per_pass is 16 at most)
             if (!mbar_wait(tfull_bar(acc), ((uint32_t)p >> 1) & 1u, s_abort, DEV_TIMEOUT_TMEM_FULL, acc)) break;
             tc_fence_after();
             for (int i = 0; i < n; ++i) {
                 const int4 req = s_req[req0 + i];
                 const float scale = __shfl_sync(0xffffffffu, scales, i);
-                const bool mine = row >= req.y && row < req.z;
-                uint4* dst = reinterpret_cast<uint4*>(a.h + ((int64_t)(tile + req.x) * a.tile_rows + (row - t0)) * a.r);
+                const bool mine = row >= req.x && row < req.y;
+                uint4* dst = reinterpret_cast<uint4*>(a.h + (int64_t)row * a.r);
                 for (int c = 0; c < a.r; c += 8) {
                     uint32_t v[8];
                     tmem_ld8(tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * kDownCols + i * a.r + c), v);
                     tmem_wait_ld();
-                    // rows of other requests are zeros, whatever their products are
-                    dst[c >> 3] = mine ? make_uint4(pack_h2(__uint_as_float(v[0]) * scale, __uint_as_float(v[1]) * scale), pack_h2(__uint_as_float(v[2]) * scale, __uint_as_float(v[3]) * scale),
-                                                    pack_h2(__uint_as_float(v[4]) * scale, __uint_as_float(v[5]) * scale), pack_h2(__uint_as_float(v[6]) * scale, __uint_as_float(v[7]) * scale))
-                                       : make_uint4(0u, 0u, 0u, 0u);
+                    if (mine)
+                        dst[c >> 3] = make_uint4(pack_h2(__uint_as_float(v[0]) * scale, __uint_as_float(v[1]) * scale), pack_h2(__uint_as_float(v[2]) * scale, __uint_as_float(v[3]) * scale),
+                                                 pack_h2(__uint_as_float(v[4]) * scale, __uint_as_float(v[5]) * scale), pack_h2(__uint_as_float(v[6]) * scale, __uint_as_float(v[7]) * scale));
                 }
             }
             tc_fence_before();
@@ -309,21 +295,18 @@ static AdapterForm adapter_form(int64_t M, int N, int K, bool swiglu, int r, int
 }
 
 // Workspace: h, or the rows form's delta.
-static int64_t adapter_space(const AdapterForm& f, int64_t M, int N, int r, int S) {
-    const int64_t tile_rows = f.pairs ? 2 * BM : BM, n_tiles = (M + tile_rows - 1) / tile_rows;
-    return f.rows ? M * N * (int64_t)sizeof(float) : (n_tiles + S) * tile_rows * r * 2;
-}
+static int64_t adapter_space(const AdapterForm& f, int64_t M, int N, int r) { return f.rows ? M * N * (int64_t)sizeof(float) : M * r * 2; }
 
 int64_t adapter_linear_workspace_bytes(int64_t M, int N, int K, int epilogue, int r, int S) {
     if (M <= 0 || S <= 0) return 0;
-    return adapter_space(adapter_form(M, N, K, epilogue == FBB_EPI_SWIGLU, r, S), M, N, r, S);
+    return adapter_space(adapter_form(M, N, K, epilogue == FBB_EPI_SWIGLU, r, S), M, N, r);
 }
 
 template <int BN, bool SWIGLU, bool CTA2, AdaptMode ADAPT>
 static int launch_adapter_variant(const CUtensorMap& ta, const CUtensorMap& tw, const CUtensorMap& th, const CUtensorMap& tu, const CUtensorMap& tc, GemmArgs g,
                                   const AdaptArgs& ad, cudaStream_t stream) {
     using S = GemmSmem<BN, CTA2>;
-    constexpr int kDynamic = S::kDynamic + 4 * S::kStages;  // and a number per stage
+    constexpr int kDynamic = S::kDynamic + 12 * S::kStages;  // and three numbers per stage
     auto kern = linear_adapter_kernel<BN, SWIGLU, CTA2, ADAPT>;
     static bool configured[64] = {};
     int dev = 0;
@@ -351,19 +334,15 @@ int launch_adapter_linear(const void* A, const void* W, void* C, const void* bia
                           const int* offsets, int S, void* ws, int64_t ws_bytes, cudaStream_t stream) {
     const bool swiglu = epilogue == FBB_EPI_SWIGLU;
     const AdapterForm f = adapter_form(M, N, K, swiglu, r, S);
-    const int64_t need = adapter_space(f, M, N, r, S);
+    const int64_t need = adapter_space(f, M, N, r);
     if (ws == nullptr || ws_bytes < need)
         return fail(FBB_ERR_SHAPE, "adapter_linear: workspace of %lld bytes, %lld needed", (long long)(ws != nullptr ? ws_bytes : 0), (long long)need);
-    const int tile_rows = f.pairs ? 2 * BM : BM;
-    const int64_t h_rows = ((M + tile_rows - 1) / tile_rows + S) * tile_rows;
-    if (h_rows > 0x7FFFFFFFll) return fail(FBB_ERR_SHAPE, "adapter_linear: too many requests (%d) for %lld rows", S, (long long)M);
 
     AdapterArgs d = {};
     d.requests.ids = ids, d.requests.offsets = offsets;
     d.requests.S = S, d.requests.each = offsets != nullptr ? 0 : (int)(M / S), d.requests.M = (int)M, d.requests.L = L;
     d.scale = scale;
     d.M = (int)M, d.N = N, d.K = K, d.r = r;
-    d.tile_rows = tile_rows;
     d.h = reinterpret_cast<__half*>(ws);
     d.x = reinterpret_cast<const __half*>(A);
     d.ldx = lda;
@@ -386,7 +365,7 @@ int launch_adapter_linear(const void* A, const void* W, void* C, const void* bia
         {&ta, A, (uint64_t)K, (uint64_t)M, lda, BK, BM, CU_TENSOR_MAP_SWIZZLE_128B},
         {&tw, W, (uint64_t)K, (uint64_t)N, ldw, BK, w_rows, CU_TENSOR_MAP_SWIZZLE_128B},
         {&tc, C, (uint64_t)(swiglu ? N / 2 : N), (uint64_t)M, ldc, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B},
-        {&th, ws, (uint64_t)r, (uint64_t)h_rows, r, BK, BM, CU_TENSOR_MAP_SWIZZLE_128B},
+        {&th, ws, (uint64_t)r, (uint64_t)M, r, BK, BM, CU_TENSOR_MAP_SWIZZLE_128B},
         {&tu, up, (uint64_t)r, (uint64_t)L * (uint64_t)N, r, BK, w_rows, CU_TENSOR_MAP_SWIZZLE_128B},
         {&td, down, (uint64_t)K, (uint64_t)L * (uint64_t)r, K, BK, (uint32_t)r, CU_TENSOR_MAP_SWIZZLE_128B}};
     for (int i = 0; i < (f.rows ? 3 : 6); ++i) {

@@ -322,7 +322,7 @@ int fbb_diff64_f16(const void* q, const void* k, const void* v, void* o, int B, 
                    int64_t q_sh, int64_t k_sb, int64_t k_sn, int64_t k_sh, int64_t v_sb, int64_t v_sn, int64_t v_sh, int64_t o_sb, int64_t o_sn,
                    int64_t o_sh, const float* lam, int64_t lam_sb, int64_t lam_sn, int64_t lam_sh, const void* weight, int weight_dtype, float eps,
                    float out_scale, float scale, const int* lengths, void* workspace, int64_t workspace_bytes, void* stream) {
-    if (B < 0 || Nq < 0 || Nk < 0 || H <= 0 || Hk <= 0 || H % Hk != 0 || (int64_t)B * H > 0x7FFFFFFFll || H > 65535)
+    if (B < 0 || Nq < 0 || Nk < 0 || Nq > (1 << 30) || Nk > (1 << 30) || H <= 0 || Hk <= 0 || H % Hk != 0 || (int64_t)B * H > 0x7FFFFFFFll || H > 65535)
         return fail(FBB_ERR_SHAPE, "diff64: bad B/Nq/Nk/H/Hk (%d, %d, %d, %d, %d)", B, Nq, Nk, H, Hk);
     if (weight != nullptr && weight_dtype != FBB_DTYPE_F16 && weight_dtype != FBB_DTYPE_F32) return fail(FBB_ERR_ENUM, "diff64: weight dtype %d", weight_dtype);
     if (!(scale > 0.f) || !(eps >= 0.f)) return fail(FBB_ERR_SHAPE, "diff64: scale must be > 0 and eps >= 0");

@@ -347,6 +347,29 @@ __device__ __forceinline__ void umma_kblock_commit_warp(uint32_t d_tmem, uint64_
         ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(bar)
         : "memory");
 }
+// The same into some rows of the accumulator only: bit i of off[w] set leaves lane 32 w + i of tensor memory as it is, whatever the operands
+// hold there. Always accumulates.
+__device__ __forceinline__ void umma_kblock_rows_commit_warp(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, const uint32_t* off, uint32_t bar) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred q;\n\t"
+        ".reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
+        "add.s64 a1, %1, 2;\n\t"
+        "add.s64 b1, %2, 2;\n\t"
+        "add.s64 a2, %1, 4;\n\t"
+        "add.s64 b2, %2, 4;\n\t"
+        "add.s64 a3, %1, 6;\n\t"
+        "add.s64 b3, %2, 6;\n\t"
+        "elect.sync _|q, 0xFFFFFFFF;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %7}, 1;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, {%4, %5, %6, %7}, 1;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, {%4, %5, %6, %7}, 1;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, {%4, %5, %6, %7}, 1;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%8];\n\t"
+        "}\n"
+        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3]), "r"(bar)
+        : "memory");
+}
 // The same with commits to two barriers, accumulator overwritten (the Q K^T of one key block).
 __device__ __forceinline__ void umma_kblock_commit2_warp(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t bar0, uint32_t bar1) {
     asm volatile(
@@ -489,6 +512,33 @@ __device__ __forceinline__ void umma_kblock_commit_pair_warp(uint32_t d_tmem, ui
         "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%5], m;\n\t"
         "}\n"
         ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(bar), "r"(mask)
+        : "memory");
+}
+// The same into some rows of the accumulator only: bit i of off[w] set leaves lane 32 w + i of tensor memory (off[0..3]: the leader's 128
+// lanes, off[4..7]: the peer's) as it is, whatever the operands hold there. Always accumulates.
+__device__ __forceinline__ void umma_kblock_rows_commit_pair_warp(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, const uint32_t* off, uint32_t bar,
+                                                                  uint32_t mask) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred q;\n\t"
+        ".reg .b16 m;\n\t"
+        ".reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
+        "add.s64 a1, %1, 2;\n\t"
+        "add.s64 b1, %2, 2;\n\t"
+        "add.s64 a2, %1, 4;\n\t"
+        "add.s64 b2, %2, 4;\n\t"
+        "add.s64 a3, %1, 6;\n\t"
+        "add.s64 b3, %2, 6;\n\t"
+        "cvt.u16.u32 m, %13;\n\t"
+        "elect.sync _|q, 0xFFFFFFFF;\n\t"
+        "@q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %7, %8, %9, %10, %11}, 1;\n\t"
+        "@q tcgen05.mma.cta_group::2.kind::f16 [%0], a1, b1, %3, {%4, %5, %6, %7, %8, %9, %10, %11}, 1;\n\t"
+        "@q tcgen05.mma.cta_group::2.kind::f16 [%0], a2, b2, %3, {%4, %5, %6, %7, %8, %9, %10, %11}, 1;\n\t"
+        "@q tcgen05.mma.cta_group::2.kind::f16 [%0], a3, b3, %3, {%4, %5, %6, %7, %8, %9, %10, %11}, 1;\n\t"
+        "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%12], m;\n\t"
+        "}\n"
+        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3]), "r"(off[4]), "r"(off[5]), "r"(off[6]), "r"(off[7]), "r"(bar),
+          "r"(mask)
         : "memory");
 }
 // The four K16 steps alone.

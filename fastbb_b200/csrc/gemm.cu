@@ -160,7 +160,7 @@ struct Requests {
 struct AdaptArgs {
     Requests requests;
     // blocks
-    const CUtensorMap* map_h;  // h of request s in tile t from row (t + s) * tile rows on, rows of other requests zero
+    const CUtensorMap* map_h;  // h [M, r]
     const CUtensorMap* map_up; // the adapters' second matrices [adapters * N, r]
     int r_blocks;              // 64-element k-blocks of the rank
     // rows
@@ -190,8 +190,9 @@ __device__ __forceinline__ void linear_umma_body(const CUtensorMap& tmap_a, cons
     auto tempty_bar = [&](int a) { return bar0 + 8u * (2 * kStages + 2 + a); };
     volatile uint32_t* s_tmem = reinterpret_cast<volatile uint32_t*>(gen + S::kBarOffset + S::kNumBars * 8);
     volatile int* s_abort = reinterpret_cast<volatile int*>(gen + S::kBarOffset + S::kNumBars * 8 + 4);
-    // (adapters) of the stage with a tile's last k-block of x and W: how many more the tile has
+    // (adapters) of the stage with a tile's last k-block of x and W: how many more the tile has; of those behind it: their request's rows
     volatile int* s_extra = reinterpret_cast<volatile int*>(gen + S::kBytes);
+    volatile int* s_rows = s_extra + kStages;  // [stage][2], relative to the tile
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
@@ -259,9 +260,9 @@ __device__ __forceinline__ void linear_umma_body(const CUtensorMap& tmap_a, cons
                 int m0, n0, w;
                 item_at(item, m0, n0, w);
                 const int nt = n0 / kOutCols;
-                // the requests of the tile's rows, the adapters of the first 32, and how many have one
+                // the requests of the tile's rows, the adapters and rows of the first 32, and how many have one
                 const int tile = item / g.tiles_n, r0 = tile * kTileRows, r1 = min(r0 + kTileRows, g.M);
-                int first = 0, end = 0, slot0 = -1, extra = 0;
+                int first = 0, end = 0, slot0 = -1, b0 = 0, e0 = 0, extra = 0;
                 auto load = [&](int kb) -> bool {
                     if (__all_sync(0xffffffffu, mbar_wait(empty_bar(s), ph ^ 1u, s_abort, DEV_TIMEOUT_SMEM_EMPTY, s)) == 0) return false;
                     const uint32_t sa = base + s * S::kStageBytes;
@@ -293,7 +294,10 @@ __device__ __forceinline__ void linear_umma_body(const CUtensorMap& tmap_a, cons
                     ad.requests.of_rows(r0, r1, lane, first, end);
                     for (int s0 = first; s0 < end; s0 += 32) {
                         const int of = s0 + lane < end ? ad.requests.adapter_in(s0 + lane, r0, r1) : -1;
-                        if (s0 == first) slot0 = of;
+                        if (s0 == first) {
+                            slot0 = of;
+                            if (of >= 0) b0 = ad.requests.begin(s0 + lane), e0 = ad.requests.begin(s0 + lane + 1);
+                        }
                         extra += __popc(__ballot_sync(0xffffffffu, of >= 0));
                     }
                     // (the stage is free: the issuer reads a stage's number before it multiplies what is in it)
@@ -303,16 +307,23 @@ __device__ __forceinline__ void linear_umma_body(const CUtensorMap& tmap_a, cons
                     ok = load(plain_kb);
                 }
                 if constexpr (ADAPT == kAdaptBlocks) {
-                    // the adapters of the tile's requests: k-blocks of h (zero outside the request's rows) and of the adapter's second matrix
+                    // the adapters of the tile's requests: k-blocks of h and of the adapter's second matrix, for the request's rows
                     for (int s0 = first; s0 < end && ok; s0 += 32) {
-                        const int slot = s0 == first ? slot0 : (s0 + lane < end ? ad.requests.adapter_in(s0 + lane, r0, r1) : -1);
+                        int slot = slot0, begin = b0, behind = e0;
+                        if (s0 != first) {
+                            slot = s0 + lane < end ? ad.requests.adapter_in(s0 + lane, r0, r1) : -1;
+                            if (slot >= 0) begin = ad.requests.begin(s0 + lane), behind = ad.requests.begin(s0 + lane + 1);
+                        }
                         for (uint32_t todo = __ballot_sync(0xffffffffu, slot >= 0); todo != 0u && ok; todo &= todo - 1u) {
                             const int i = __ffs(todo) - 1;
-                            const int up0 = __shfl_sync(0xffffffffu, slot, i) * g.N, h0 = (tile + s0 + i) * kTileRows + (int)rank * BM;
+                            const int up0 = __shfl_sync(0xffffffffu, slot, i) * g.N;
+                            const int b = max(__shfl_sync(0xffffffffu, begin, i), r0) - r0, e = min(__shfl_sync(0xffffffffu, behind, i), r1) - r0;
                             for (int kb = 0; kb < ad.r_blocks; ++kb) {
                                 if (__all_sync(0xffffffffu, mbar_wait(empty_bar(s), ph ^ 1u, s_abort, DEV_TIMEOUT_SMEM_EMPTY, s)) == 0) { ok = false; break; }
                                 const uint32_t sa = base + s * S::kStageBytes;
                                 const uint32_t sb = sa + S::kABytes;
+                                if (lane == 0) s_rows[2 * s] = b, s_rows[2 * s + 1] = e;
+                                __syncwarp();
                                 // the second matrix needs nothing of the kernel that makes h
                                 if constexpr (CTA2) {
                                     const int wrow = SWIGLU ? (rank == 0 ? nt * (BN / 2) : g.N / 2 + nt * (BN / 2)) : nt * BN + (int)rank * (BN / 2);
@@ -320,14 +331,14 @@ __device__ __forceinline__ void linear_umma_body(const CUtensorMap& tmap_a, cons
                                     __syncwarp();
                                     tma_load_2d_pair_warp(sb, ad.map_up, full_bar(s), kb * BK, up0 + wrow);
                                     grid_dependency_wait();
-                                    tma_load_2d_pair_warp(sa, ad.map_h, full_bar(s), kb * BK, h0);
+                                    tma_load_2d_pair_warp(sa, ad.map_h, full_bar(s), kb * BK, m0);
                                 } else {
                                     if (lane == 0) mbar_arrive_expect_tx(full_bar(s), S::kStageBytes);
                                     __syncwarp();
                                     tma_load_2d_warp(sb, ad.map_up, full_bar(s), kb * BK, up0 + (SWIGLU ? nt * (BN / 2) : nt * BN));
                                     if (SWIGLU) tma_load_2d_warp(sb + S::kBBytes / 2, ad.map_up, full_bar(s), kb * BK, up0 + g.N / 2 + nt * (BN / 2));
                                     grid_dependency_wait();
-                                    tma_load_2d_warp(sa, ad.map_h, full_bar(s), kb * BK, h0);
+                                    tma_load_2d_warp(sa, ad.map_h, full_bar(s), kb * BK, m0);
                                 }
                                 if (++s == kStages) { s = 0; ph ^= 1u; }
                             }
@@ -378,7 +389,23 @@ __device__ __forceinline__ void linear_umma_body(const CUtensorMap& tmap_a, cons
                 if (!ok) break;
                 const int extra = s_extra[s];
                 ok = multiply(plain_kb);
-                for (int kb = 0; kb < extra && ok; ++kb) ok = multiply(1);
+                for (int kb = 0; kb < extra && ok; ++kb) {
+                    ok = all_ok(mbar_wait(full_bar(s), ph, s_abort, DEV_TIMEOUT_TMA_FULL, s));
+                    if (!ok) break;
+                    tc_fence_after();
+                    // Into the request's rows alone: others' rows hold others' h, and an infinity in one adapter is none of theirs.
+                    const int b = s_rows[2 * s], e = s_rows[2 * s + 1];
+                    uint32_t off[CTA2 ? 8 : 4];
+#pragma unroll
+                    for (int i = 0; i < (CTA2 ? 8 : 4); ++i) {
+                        const int lo = min(max(b - 32 * i, 0), 32), hi = min(max(e - 32 * i, 0), 32);  // rows [lo, hi) of these 32 are the request's
+                        off[i] = ~(uint32_t)((1ull << hi) - (1ull << min(lo, hi)));
+                    }
+                    const uint64_t adesc = adesc0 + (uint64_t)(s * (S::kStageBytes >> 4)), bdesc = adesc + (uint64_t)(S::kABytes >> 4);
+                    if constexpr (CTA2) umma_kblock_rows_commit_pair_warp(d_tmem, adesc, bdesc, idesc, off, empty_bar(s), 3u);
+                    else umma_kblock_rows_commit_warp(d_tmem, adesc, bdesc, idesc, off, empty_bar(s));
+                    if (++s == kStages) { s = 0; ph ^= 1u; }
+                }
             }
             if (!ok) break;
             if constexpr (CTA2) umma_commit_pair_warp(tfull_bar(acc));  // both CTAs' accumulators complete

@@ -127,15 +127,32 @@ def test_without_any_adapter_it_is_the_linear_layer():
 
 
 @pytest.mark.gpu
-def test_infinite_values_stay_in_their_rows():
-    """A request's NaN and infinities (in x or its adapter) reach only its rows: the k-blocks of other requests hold zeros there."""
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("M,N,bounds", [(300, 256, [0, 100, 130, 300]), (3000, 1024, [0, 1000, 1033, 3000]), (40, 512, [0, 1, 2, 40])])
+def test_infinite_values_stay_in_their_rows(M, N, bounds, bad):
+    """A request's NaN and infinities, in its rows of x or in its adapter, reach only its rows, though tiles hold several requests."""
     g = torch.Generator("cuda").manual_seed(5)
-    bounds, ids = [0, 100, 130, 300], [0, 1, 0]
-    x, w, slots, b = make(300, 128, 256, 16, 2, g)
+    ids = [0, 1, 0]
+    x, w, slots, b = make(M, 128, N, 16, 2, g)
+    rows = slice(bounds[1], bounds[2])
     clean = adapter_linear(x, w, slots, vector(ids), vector(bounds), b=b)
-    x[100:130, 5] = float("nan")
-    out = adapter_linear(x, w, slots, vector(ids), vector(bounds), b=b)
-    assert torch.equal(out[:100], clean[:100]) and torch.equal(out[130:], clean[130:]) and bool(out[100:130].isnan().all())
+
+    def others_are_clean():
+        out = adapter_linear(x, w, slots, vector(ids), vector(bounds), b=b)
+        assert torch.equal(out[:rows.start], clean[:rows.start]) and torch.equal(out[rows.stop:], clean[rows.stop:])
+        return out[rows]
+
+    kept = x[rows, 5].clone()
+    x[rows, 5] = bad
+    assert not bool(others_are_clean().isfinite().any())
+    x[rows, 5] = kept
+    for matrix in (slots.up, slots.down):
+        kept_matrix = matrix[1].clone()
+        matrix[1] = bad
+        assert not bool(others_are_clean().isfinite().any())
+        matrix[1] = kept_matrix
+    slots.scale[1] = bad
+    assert not bool(others_are_clean().isfinite().any())
 
 
 @pytest.mark.gpu

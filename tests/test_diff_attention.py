@@ -101,6 +101,19 @@ def test_keys_beyond_a_length_are_not_seen(Nq, Nk, lengths, bad):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("B,Nq,Nk,H", [(7, 700, 700, 6), (40, 150, 200, 4), (33, 1, 300, 2)])
+def test_many_tiles_of_uneven_lengths(B, Nq, Nk, H):
+    """More tiles than SMs, some of no keys, their entries in no order; more entries than a warp has lanes."""
+    g = torch.Generator("cuda").manual_seed(B)
+    q, k, v, lam = make(B, Nq, Nk, H, H // 2, g)
+    lengths = [(37 * i * i + 11) % (Nk + 1) if i % 3 else 0 for i in range(B)]
+    weight = torch.randn(128, generator=g, device="cuda").half()
+    n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    check(diff_attention(q, k, v, lam, weight=weight, key_lengths=n), q, k, v, lam, weight=weight, lengths=lengths)
+    assert _lib.device_status() == (0, 0, 0, 0)
+
+
+@pytest.mark.gpu
 def test_no_keys_at_all():
     g = torch.Generator("cuda").manual_seed(1)
     q, k, v, lam = make(2, 5, 0, 2, 2, g)
