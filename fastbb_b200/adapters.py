@@ -24,7 +24,7 @@ class Adapters:
         if not (down.is_cuda and down.dtype == up.dtype == torch.float16 and down.device == up.device and down.dim() == up.dim() == 3):
             raise ValueError("down [L, r, K] and up [L, N, r] must be fp16 tensors on one GPU (there is no CPU path)")
         count, rank, k = down.shape
-        if up.shape[0] != count or up.shape[2] != rank or count < 1:
+        if up.shape[0] != count or up.shape[2] != rank or min(count, k, up.shape[1]) < 1:
             raise ValueError(f"down {tuple(down.shape)} and up {tuple(up.shape)} do not hold the same adapters")
         if rank < 8 or rank > 128 or rank % 8:
             raise ValueError(f"the rank must be a multiple of 8 up to 128, got {rank}: pad with zeros")

