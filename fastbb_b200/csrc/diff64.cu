@@ -28,6 +28,8 @@
 // Bound by the exponentials where tiles are many: 6145 queries x 8 heads take 234 us, 993 TFLOP/s, with the transcendental unit busy for
 // 71 % of the clocks an SM is active and the tensor pipe for 54 %; few queries by the read of K and V (1 x 16385 x 8: 23 us, 10 of them
 // the read). Short tiles pay for their ends: 6.6 k clocks behind 2.8 k a block.
+#include <cfloat>
+
 #include "common.cuh"
 #include "internal.h"
 
@@ -408,7 +410,8 @@ diff64_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
                 if (rowB < a.Nq) lamB = lam[rowB * a.l_sn];
             }
             float tA = 0.f, tB = 0.f;
-            float mA = -INFINITY, mB = -INFINITY, lA = 0.f, lB = 0.f;
+            // (no lower: the maximum of keys that are all at minus infinity is subtracted from it)
+            float mA = -FLT_MAX, mB = -FLT_MAX, lA = 0.f, lB = 0.f;
             auto unit = [&](int i) -> bool {  // one half-block
                 const uint32_t half = g & 1u, tSh = tS + 64u * half;
                 if (!mbar_wait(s_full(t, half), (g >> 1) & 1u, s_abort, DEV_TIMEOUT_TMEM_FULL, 2 * t + half)) return false;

@@ -206,6 +206,24 @@ def test_with_one_map_off_it_is_attention():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("Nq,Nk,dead", [(200, 300, 64), (200, 300, 299), (1, 4000, 700), (5, 129, 128), (3, 4000, 3999)])
+def test_scores_of_minus_infinity_ahead_of_the_others(Nq, Nk, dead):
+    """Keys that an infinity in them takes out of every row's maps have no weight, whole blocks and shares of them too; a row of nothing else is NaN."""
+    g = torch.Generator("cuda").manual_seed(dead)
+    q, k, v, lam = make(2, Nq, Nk, 2, 2, g)
+    q[..., 5] = 0.5 + q[..., 5].abs()
+    kept = slice(dead, Nk)
+    k[:, :dead, :, 5] = -float("inf")
+    out = diff_attention(q, k, v, lam)
+    check(out, q, k[:, kept], v[:, kept], lam)
+    k[1, :, :, 5] = -float("inf")
+    out = diff_attention(q, k, v, lam)
+    assert bool(out[1].isnan().all())
+    check(out[:1], q[:1], k[:1, kept], v[:1, kept], lam)
+    assert _lib.device_status() == (0, 0, 0, 0)
+
+
+@pytest.mark.gpu
 def test_refusals_on_the_gpu():
     g = torch.Generator("cuda").manual_seed(7)
     q, k, v, lam = make(2, 20, 30, 4, 2, g)
