@@ -666,7 +666,7 @@ __global__ void __launch_bounds__(512) diff64_join_kernel(const DiffArgs a) {
     const float4 y0 = *reinterpret_cast<const float4*>(&s_o[r][c]), y1 = *reinterpret_cast<const float4*>(&s_o[r][c + 4]);
     float o[8] = {x[0][0].x - y0.x, x[0][0].y - y0.y, x[0][0].z - y0.z, x[0][0].w - y0.w, x[0][1].x - y1.x, x[0][1].y - y1.y, x[0][1].z - y1.z, x[0][1].w - y1.w};
     float scale = a.out_scale;
-    if (a.weight != nullptr) {
+    if (a.weight != nullptr && live > 0) {  // (a row without keys is 0, with an eps of 0 too)
         const unsigned mask = 0xffffu << (threadIdx.x & 16);
         float sum = 0.f;
 #pragma unroll

@@ -206,6 +206,20 @@ def test_with_one_map_off_it_is_attention():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("Nq,Nk", [(3, 4000), (200, 300)])
+def test_rows_without_keys_are_zero_with_a_norm_of_no_epsilon(Nq, Nk):
+    """Few queries over many keys (two launches) and tiles of one launch alike."""
+    g = torch.Generator("cuda").manual_seed(Nq)
+    q, k, v, lam = make(3, Nq, Nk, 2, 2, g)
+    weight = torch.randn(128, generator=g, device="cuda").half()
+    lengths = [Nk, 0, 70]
+    n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    out = diff_attention(q, k, v, lam, weight=weight, eps=0.0, key_lengths=n)
+    assert bool((out[1] == 0).all())
+    check(out[::2], q[::2], k[::2], v[::2], lam, weight=weight, eps=0.0, lengths=lengths[::2])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("Nq,Nk,dead", [(200, 300, 64), (200, 300, 299), (1, 4000, 700), (5, 129, 128), (3, 4000, 3999)])
 def test_scores_of_minus_infinity_ahead_of_the_others(Nq, Nk, dead):
     """Keys that an infinity in them takes out of every row's maps have no weight, whole blocks and shares of them too; a row of nothing else is NaN."""
