@@ -98,6 +98,8 @@ def rotary(q, k, positions, plan, n_prefix=0, inverse=False, out=None):
     if plan.device != device:
         raise ValueError(f"the plan is on {plan.device}, the tensors on {device}")
     pairs, n_axes = plan.pairs, plan.n_axes
+    if B * N > 0x7FFFFFFF:
+        raise ValueError("rotary takes fewer than 2^31 tokens")
     if 2 * pairs > D:
         raise ValueError(f"the plan turns {2 * pairs} columns, a head has {D}")
     if n_prefix < 0 or n_prefix > N:

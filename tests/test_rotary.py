@@ -193,6 +193,17 @@ def test_refusals_on_the_gpu():
     assert torch.equal(rotary(q, k, where, plan, out=(v, torch.empty_like(k)))[0], q)  # another part of the buffer is fine
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,N", [(1, 2 ** 31), (1, 2 ** 32 + 1), (2 ** 16, 2 ** 15), (2 ** 32 + 1, 1)])
+def test_more_tokens_than_31_bits_count_are_refused(B, N):
+    """(Views of a single row: nothing is allocated.)"""
+    plan = axial_plan(64)
+    row, where = torch.zeros(64, dtype=torch.float16, device="cuda"), torch.zeros(2, device="cuda")
+    q = row.as_strided((B, N, 1, 64), (0, 0, 0, 1))
+    with pytest.raises(ValueError, match="2\\^31 tokens"):
+        rotary(q, None, where.as_strided((N, 2), (0, 1)), plan, out=(q, None))
+
+
 # ------------------------------------------------------------------------------------------------------------------ CPU
 def test_plans():
     plan = axial_plan(64, axes=3, theta=50.0, unit=2.0, shares=[8, 12, 12], device="cpu")
