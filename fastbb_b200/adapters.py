@@ -28,6 +28,8 @@ class Adapters:
             raise ValueError(f"down {tuple(down.shape)} and up {tuple(up.shape)} do not hold the same adapters")
         if rank < 8 or rank > 128 or rank % 8:
             raise ValueError(f"the rank must be a multiple of 8 up to 128, got {rank}: pad with zeros")
+        if max(count * max(up.shape[1], rank), k) > 0x7FFFFFFF:
+            raise ValueError("the adapters' rows, of either matrix, must number fewer than 2^31")
         if scale is None:
             scale = torch.ones(count, device=down.device)
         if scale.dtype != torch.float32 or scale.shape != (count,) or scale.device != down.device:
@@ -40,7 +42,8 @@ class Adapters:
 
 def adapter_linear(x, w, adapters, ids, offsets=None, b=None, act=None, res=None, gamma=None, out=None):
     """act(x w^T + b + scale_a (x down_a^T) up_a^T), a the adapter of the row's request; with res: res + gamma * that. As linear(): fp16 x [..., K],
-    w [N, K], b and gamma vectors, res of the output's shape, act None | "gelu" | "swiglu"; fp32 accumulator.
+    w [N, K], b and gamma vectors, res of the output's shape, act None | "gelu" | "swiglu"; fp32 accumulator. Each scale_a (x down_a^T) is rounded to
+    fp16 on the way (but for few rows of many requests): beyond fp16's range it is infinite.
 
     ids: int32 [S] on the GPU, the adapter of each request; a number out of [0, L) (say -1): none.
     offsets: int32 [S + 1] on the GPU, not decreasing: request s has rows offsets[s] .. offsets[s + 1] - 1 of x's rows taken in order; rows of

@@ -299,7 +299,8 @@ int fbb_adapter_linear_f16(const void* A, const void* W, void* C, const void* bi
     if (lda < K || ldw < K || ldc < n_out || (res != nullptr && ldr < n_out))
         return fail(FBB_ERR_SHAPE, "adapter_linear: a leading dimension is smaller than its row length");
     if (rank < 8 || rank > 128 || (rank & 7) != 0) return fail(FBB_ERR_SHAPE, "adapter_linear: rank must be a multiple of 8 from 8 to 128, got %d", rank);
-    if (adapters < 1 || (int64_t)adapters * N > 0x7FFFFFFFll) return fail(FBB_ERR_SHAPE, "adapter_linear: need 1 <= adapters and adapters * N < 2^31 (%d, %d)", adapters, N);
+    if (adapters < 1 || (int64_t)adapters * (N > rank ? N : rank) > 0x7FFFFFFFll)
+        return fail(FBB_ERR_SHAPE, "adapter_linear: need 1 <= adapters, and adapters * N and adapters * rank < 2^31 (%d, %d, %d)", adapters, N, rank);
     if (requests < 1 || (offsets == nullptr && M % requests != 0))
         return fail(FBB_ERR_SHAPE, "adapter_linear: need at least one request, and without offsets the same number of rows for each (%d for %lld rows)", requests, (long long)M);
     if (M == 0) return FBB_OK;

@@ -264,3 +264,15 @@ def test_entry_point_refusals():
     assert call(bytes_=64) == -2 and b"workspace" in lib.fbb_last_error()
     assert call(M=0, a=None) == 0
     assert lib.fbb_adapter_linear_workspace_bytes(0, 64, 64, 0, 8, 1) == 0
+
+
+def test_more_rows_of_either_matrix_than_31_bits_count_are_refused():
+    """(The workspace is the next thing that is refused: nothing is read or launched.)"""
+    lib, A = _lib.load(), 0x7F0000000000
+
+    def call(L, N, r):
+        rc = lib.fbb_adapter_linear_f16(A, A, A + (1 << 30), None, None, None, 8, N, 32, 32, 32, N, 0, 0, A, A, A, L, r, A, None, 2, A, 0, None)
+        return rc, b"2^31" in lib.fbb_last_error()
+
+    assert call(1 << 24, 8, 128) == (-2, True) and call(1 << 28, 8, 8) == (-2, True) and call(1 << 20, 1 << 14, 8) == (-2, True)
+    assert call((1 << 24) - 1, 8, 128)[1] is False
