@@ -106,10 +106,9 @@ def adapter_linear(x, w, adapters, ids, offsets=None, b=None, act=None, res=None
         lib = _lib.load()
         need = lib.fbb_adapter_linear_workspace_bytes(M, N, K, code, adapters.rank, S)
         ws = x.new_empty((need + 1) // 2)
-        _lib.check(lib.fbb_adapter_linear_f16(
-            x2.data_ptr(), w.data_ptr(), out.data_ptr(), _lib.ptr(b), _lib.ptr(r2), _lib.ptr(gamma), M, N, K, lda,
-            w.stride(0) if N > 1 else K, n_out, ldr if res is not None else 0, code, adapters.down.data_ptr(),
-            adapters.up.data_ptr(), adapters.scale.data_ptr(), adapters.count, adapters.rank, ids.data_ptr(), _lib.ptr(offsets), S, ws.data_ptr(), need,
-            _lib.stream_ptr(device)))
+        _lib.check(lib.fbb_adapter_linear_f16_from(_lib.AdapterLinearArgs.pack(
+            x2.data_ptr(), w.data_ptr(), out.data_ptr(), _lib.address(b), _lib.address(r2), _lib.address(gamma), adapters.down.data_ptr(), adapters.up.data_ptr(),
+            adapters.scale.data_ptr(), ids.data_ptr(), _lib.address(offsets), ws.data_ptr(), _lib.stream_ptr(device), M, lda, w.stride(0) if N > 1 else K, n_out,
+            ldr if res is not None else 0, need, N, K, code, adapters.count, adapters.rank, S)))
         _lib.launched(2)
     return out

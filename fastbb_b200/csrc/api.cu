@@ -316,6 +316,12 @@ int fbb_adapter_linear_f16(const void* A, const void* W, void* C, const void* bi
                                  workspace, workspace_bytes, (cudaStream_t)stream);
 }
 
+int fbb_adapter_linear_f16_from(const fbb_adapter_linear_args* a) {
+    if (a == nullptr) return fail(FBB_ERR_NULL, "adapter_linear: no arguments");
+    return fbb_adapter_linear_f16(a->A, a->W, a->C, a->bias, a->res, a->gamma, a->M, a->N, a->K, a->lda, a->ldw, a->ldc, a->ldr, a->epilogue, a->down, a->up,
+                                  a->scale, a->adapters, a->rank, a->ids, a->offsets, a->requests, a->workspace, a->workspace_bytes, a->stream);
+}
+
 int64_t fbb_diff64_workspace_bytes(int B, int Nq, int Nk, int H) { return diff64_workspace_bytes(B, Nq, Nk, H); }
 int fbb_diff64_launches(int B, int Nq, int Nk, int H) { return diff64_launches(B, Nq, Nk, H); }
 
@@ -343,6 +349,13 @@ int fbb_diff64_f16(const void* q, const void* k, const void* v, void* o, int B, 
                          workspace_bytes, (cudaStream_t)stream);
 }
 
+int fbb_diff64_f16_from(const fbb_diff64_args* a) {
+    if (a == nullptr) return fail(FBB_ERR_NULL, "diff64: no arguments");
+    return fbb_diff64_f16(a->q, a->k, a->v, a->o, a->B, a->Nq, a->Nk, a->H, a->Hk, a->q_s[0], a->q_s[1], a->q_s[2], a->k_s[0], a->k_s[1], a->k_s[2],
+                          a->v_s[0], a->v_s[1], a->v_s[2], a->o_s[0], a->o_s[1], a->o_s[2], a->lam, a->lam_s[0], a->lam_s[1], a->lam_s[2], a->weight,
+                          a->weight_dtype, a->eps, a->out_scale, a->scale, a->lengths, a->workspace, a->workspace_bytes, a->stream);
+}
+
 int fbb_rotary(const fbb_rotary_tensor* tensors, int n_tensors, int B, int N, int D, int pairs, int pairing, int n_prefix, const void* positions,
                int pos_dtype, int n_axes, int64_t p_sb, int64_t p_sn, int64_t p_sa, const float* freqs, const int* axes, int inverse, int dtype,
                void* stream) {
@@ -368,6 +381,12 @@ int fbb_rotary(const fbb_rotary_tensor* tensors, int n_tensors, int B, int N, in
     }
     return launch_rotary(tensors, n_tensors, B, N, D, pairs, pairing, n_prefix, positions, pos_dtype, n_axes, p_sb, p_sn, p_sa, freqs, axes, inverse,
                          dtype, (cudaStream_t)stream);
+}
+
+int fbb_rotary_from(const fbb_rotary_args* a) {
+    if (a == nullptr) return fail(FBB_ERR_NULL, "rotary: no arguments");
+    return fbb_rotary(a->tensors, a->n_tensors, a->B, a->N, a->D, a->pairs, a->pairing, a->n_prefix, a->positions, a->pos_dtype, a->n_axes, a->p_sb, a->p_sn,
+                      a->p_sa, a->freqs, a->axes, a->inverse, a->dtype, a->stream);
 }
 
 #endif  // FBB_FLASH_ONLY

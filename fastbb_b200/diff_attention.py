@@ -74,8 +74,9 @@ def diff_attention(q, k, v, lam, weight=None, eps=1e-5, out_scale=1.0, scale=Non
         lib = _lib.load()
         need = lib.fbb_diff64_workspace_bytes(B, Nq, Nk, H)
         ws = q.new_empty((need + 1) // 2) if need > 0 else None
-        _lib.check(lib.fbb_diff64_f16(
-            q_ptr, k_ptr, v_ptr, out.data_ptr(), B, Nq, Nk, H, Hk, *qs[:3], *ks[:3], *vs[:3], *out.stride()[:3], lam.data_ptr(), *ls, _lib.ptr(weight), _lib.DTYPE_CODE[weight.dtype] if weight is not None else 0, float(eps), float(out_scale),
-            float(scale), _lib.ptr(key_lengths), _lib.ptr(ws), need, _lib.stream_ptr(device)))
+        _lib.check(lib.fbb_diff64_f16_from(_lib.Diff64Args.pack(
+            q_ptr, k_ptr, v_ptr, out.data_ptr(), lam.data_ptr(), _lib.address(weight), _lib.address(key_lengths), _lib.address(ws), _lib.stream_ptr(device),
+            *qs[:3], *ks[:3], *vs[:3], *out.stride()[:3], *ls, need, B, Nq, Nk, H, Hk, _lib.DTYPE_CODE[weight.dtype] if weight is not None else 0,
+            eps, out_scale, scale)))
         _lib.launched(2 if need > 0 else 1)
     return out

@@ -16,6 +16,7 @@ from . import _lib
 
 _PAIRING = {"half": 0, "pairs": 1}
 _POS_CODE = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+_ABSENT = (0,) * 9  # a second tensor's fields
 
 
 class RotaryPlan:
@@ -119,15 +120,15 @@ def rotary(q, k, positions, plan, n_prefix=0, inverse=False, out=None):
     if B == 0 or N == 0:
         return result
     y, y_strides = result[0], result[0].stride()
-    tensors = (_lib.RotaryTensor * 2)()
-    tensors[0] = (q.data_ptr(), y.data_ptr(), H, *q_strides[:3], *y_strides[:3])
+    first = (q.data_ptr(), y.data_ptr(), H, *q_strides[:3], *y_strides[:3])
+    second = _ABSENT
     if k is not None:
         y, y_strides = result[1], result[1].stride()
-        tensors[1] = (k.data_ptr(), y.data_ptr(), k_shape[2], *k_strides[:3], *y_strides[:3])
+        second = (k.data_ptr(), y.data_ptr(), k_shape[2], *k_strides[:3], *y_strides[:3])
     with _lib.on(device):
-        _lib.check(_lib.load().fbb_rotary(
-            tensors, 1 if k is None else 2, B, N, D, pairs, _PAIRING[plan.pairing], n_prefix, positions.data_ptr(), pos_code, n_axes, *pos_strides,
-            plan.freqs.data_ptr(), plan.axes.data_ptr(), 1 if inverse else 0, code, _lib.stream_ptr(device)))
+        _lib.check(_lib.load().fbb_rotary_from(_lib.RotaryArgs.pack(
+            *first, *second, positions.data_ptr(), plan.freqs.data_ptr(), plan.axes.data_ptr(), _lib.stream_ptr(device), *pos_strides,
+            1 if k is None else 2, B, N, D, pairs, _PAIRING[plan.pairing], n_prefix, pos_code, n_axes, 1 if inverse else 0, code)))
     _lib.launched()
     return result
 

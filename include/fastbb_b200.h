@@ -209,6 +209,18 @@ int64_t fbb_adapter_linear_workspace_bytes(int64_t M, int N, int K, int epilogue
 int fbb_adapter_linear_f16(const void* A, const void* W, void* C, const void* bias, const void* res, const void* gamma, int64_t M, int N, int K,
                            int64_t lda, int64_t ldw, int64_t ldc, int64_t ldr, int epilogue, const void* down, const void* up, const float* scale,
                            int adapters, int rank, const int* ids, const int* offsets, int requests, void* workspace, int64_t workspace_bytes, void* stream);
+/* The same call with its arguments in a record (for callers that pay for each argument that crosses the boundary). */
+typedef struct fbb_adapter_linear_args {
+    const void *A, *W;
+    void* C;
+    const void *bias, *res, *gamma, *down, *up;
+    const float* scale;
+    const int *ids, *offsets;
+    void *workspace, *stream;
+    int64_t M, lda, ldw, ldc, ldr, workspace_bytes;
+    int32_t N, K, epilogue, adapters, rank, requests;
+} fbb_adapter_linear_args;
+int fbb_adapter_linear_f16_from(const fbb_adapter_linear_args* args);
 
 /* ---- differential attention -----------------------------------------------------------------------------------------------
  * o = softmax(scale q1 k1^T) v - lam softmax(scale q2 k2^T) v: two maps of head dimension 64 over the same values of 128 columns;
@@ -229,6 +241,20 @@ int fbb_diff64_f16(const void* q, const void* k, const void* v, void* o, int B, 
                    int64_t q_sh, int64_t k_sb, int64_t k_sn, int64_t k_sh, int64_t v_sb, int64_t v_sn, int64_t v_sh, int64_t o_sb, int64_t o_sn,
                    int64_t o_sh, const float* lam, int64_t lam_sb, int64_t lam_sn, int64_t lam_sh, const void* weight, int weight_dtype, float eps,
                    float out_scale, float scale, const int* lengths, void* workspace, int64_t workspace_bytes, void* stream);
+/* The same call with its arguments in a record; q_s and the others: batch, token, head. */
+typedef struct fbb_diff64_args {
+    const void *q, *k, *v;
+    void* o;
+    const float* lam;
+    const void* weight;
+    const int* lengths;
+    void *workspace, *stream;
+    int64_t q_s[3], k_s[3], v_s[3], o_s[3], lam_s[3], workspace_bytes;
+    int32_t B, Nq, Nk, H, Hk, weight_dtype;
+    float eps, out_scale, scale;
+    int32_t unused;
+} fbb_diff64_args;
+int fbb_diff64_f16_from(const fbb_diff64_args* args);
 
 /* ---- rotary positions ---------------------------------------------------------------------------------------------------
  * Queries and keys turned by the positions of their tokens on one or several axes, one launch for both. No counterpart in the
@@ -253,6 +279,17 @@ typedef struct fbb_rotary_tensor {
 int fbb_rotary(const fbb_rotary_tensor* tensors, int n_tensors, int B, int N, int D, int pairs, int pairing, int n_prefix, const void* positions,
                int pos_dtype, int n_axes, int64_t p_sb, int64_t p_sn, int64_t p_sa, const float* freqs, const int* axes, int inverse, int dtype,
                void* stream);
+/* The same call with its arguments in a record. */
+typedef struct fbb_rotary_args {
+    fbb_rotary_tensor tensors[2];
+    const void* positions;
+    const float* freqs;
+    const int* axes;
+    void* stream;
+    int64_t p_sb, p_sn, p_sa;
+    int32_t n_tensors, B, N, D, pairs, pairing, n_prefix, pos_dtype, n_axes, inverse, dtype, unused;
+} fbb_rotary_args;
+int fbb_rotary_from(const fbb_rotary_args* args);
 
 /* ---- one FFI crossing per transformer block or per run of blocks -------------------------------------------------------
  * Replaces FastViT.block / block_chunked and the loop over blocks in FastViT.run (fastbb/vit.py:108-172, 175-187), which

@@ -276,3 +276,19 @@ def test_more_rows_of_either_matrix_than_31_bits_count_are_refused():
 
     assert call(1 << 24, 8, 128) == (-2, True) and call(1 << 28, 8, 8) == (-2, True) and call(1 << 20, 1 << 14, 8) == (-2, True)
     assert call((1 << 24) - 1, 8, 128)[1] is False
+
+
+def test_the_record_form_refuses_what_the_other_does():
+    """Every field is where the entry point looks for it: broken alone, it is the one that is named."""
+    lib, A = _lib.load(), 0x7F0000000000
+    good = dict(a=A, w=A, c=A + (1 << 30), b=A, res=A, gamma=A, down=A, up=A, scale=A, ids=A, offsets=A, ws=A, stream=0, M=8, lda=32, ldw=32, ldc=64, ldr=64,
+                bytes_=0, N=64, K=32, epi=0, L=2, r=16, S=3)
+
+    def call(**kw):
+        return lib.fbb_adapter_linear_f16_from(_lib.AdapterLinearArgs.pack(*{**good, **kw}.values()))
+
+    assert lib.fbb_adapter_linear_f16_from(None) == call(a=0) == call(w=0) == call(c=0) == call(down=0) == call(up=0) == call(scale=0) == call(ids=0) == -1
+    assert call(offsets=0) == call(M=-1) == call(K=12) == call(N=12) == call(lda=24) == call(ldw=24) == call(ldc=56) == call(ldr=8) == call(c=A) == -2
+    assert call(r=12) == call(L=0) == call(S=0) == call(epi=2) == -2 and call(epi=3) == -4 and call(epi=2, res=0) == -2
+    assert call(res=A + 8) == call(up=A + 8) == call(down=A + 8) == call(ws=A + 128) == -3
+    assert call(bytes_=64) == -2 and b"workspace of 64 bytes" in lib.fbb_last_error() and call(M=0, a=0) == 0

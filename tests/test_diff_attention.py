@@ -283,3 +283,19 @@ def test_entry_point_refusals():
     assert call(wd=1) == call(wd=7) == -4
     assert call(B=0, q=None) == call(Nq=0, o=None) == 0
     assert lib.fbb_diff64_workspace_bytes(0, 1, 1000, 8) == 0 and lib.fbb_diff64_launches(1, 0, 10, 2) == 0
+
+
+def test_the_record_form_refuses_what_the_other_does():
+    """Every field is where the entry point looks for it: broken alone, it is the one that is named."""
+    lib, A = _lib.load(), 0x7F0000000000
+    good = dict(q=A, k=A, v=A, o=A, lam=A, weight=A, lengths=A, ws=0, stream=0, **{f"s{i}": n for i, n in enumerate((2048, 512, 64, 2048, 256, 64, 2048, 256, 128, 2048, 512, 128))},
+                l0=0, l1=0, l2=1, need=0, B=2, Nq=4, Nk=6, H=4, Hk=2, wd=0, eps=1e-5, out_scale=1.0, scale=0.125)
+
+    def call(**kw):
+        return lib.fbb_diff64_f16_from(_lib.Diff64Args.pack(*{**good, **kw}.values()))
+
+    assert lib.fbb_diff64_f16_from(None) == call(q=0) == call(k=0) == call(v=0) == call(o=0) == call(lam=0) == -1
+    assert call(B=-1) == call(Nq=-1) == call(Nk=-1) == call(H=0) == call(Hk=3) == call(scale=0.0) == call(eps=-1.0) == -2 and call(wd=7) == -4
+    assert [call(**{f"s{i}": 12}) for i in range(12)] == [-3] * 12 and call(ws=A + 4) == -3 and call(weight=0, wd=7, Nq=0) == call(B=0, q=0) == 0
+    many = dict(B=1, Nq=1, Nk=4096, H=1, Hk=1)  # (split over the keys: the workspace is asked for)
+    assert call(**many, ws=A, need=lib.fbb_diff64_workspace_bytes(1, 1, 4096, 1) - 1) == -2 and b"workspace" in lib.fbb_last_error()

@@ -257,3 +257,18 @@ def test_entry_point_refusals():
     assert call(x=A + 1) == call(y=A + 2, dtype=2) == call(pos=A + 4, pd=1) == -3
     assert call(pairing=2) == call(pd=3) == call(dtype=4) == -4
     assert call(B=0, x=None) == call(N=0, pos=None) == 0
+
+
+def test_the_record_form_refuses_what_the_other_does():
+    """Every field is where the entry point looks for it: broken alone, it is the one that is named."""
+    lib, A = _lib.load(), 0x7F0000000000
+    good = dict(x0=A, y0=A, h0=2, **{f"s{i}": 64 for i in range(6)}, x1=A, y1=A, h1=2, **{f"t{i}": 64 for i in range(6)}, pos=A, freqs=A, ax=A, stream=0,
+                p0=0, p1=2, p2=1, n=2, B=1, N=4, D=64, pairs=32, pairing=0, prefix=0, pd=2, axes=2, inverse=0, dtype=0)
+
+    def call(**kw):
+        return lib.fbb_rotary_from(_lib.RotaryArgs.pack(*{**good, **kw}.values()))
+
+    assert lib.fbb_rotary_from(None) == call(x0=0) == call(y0=0) == call(x1=0) == call(y1=0) == call(freqs=0) == call(ax=0) == call(pos=0) == -1
+    assert call(h0=0) == call(h1=0) == call(n=3) == call(D=1026) == call(pairs=33) == call(axes=0) == call(prefix=-1) == call(N=-1) == call(B=-1) == -2
+    assert call(y1=A + 1) == call(y0=A + 2, dtype=2) == call(pos=A + 4, pd=1) == -3 and call(pairing=2) == call(pd=3) == call(dtype=4) == -4
+    assert call(B=0, x0=0) == call(N=0, x1=0) == call(n=1, B=0, h1=0) == 0
