@@ -164,16 +164,20 @@ def address(t):
     return t.data_ptr() if t is not None else 0
 
 
+def _nest(dims, span):
+    """Whether every one of dims, (stride, size) innermost first, steps over what the dimensions inside it span, from `span` elements on."""
+    for s, n in dims:
+        if s < span:
+            return False
+        span += (n - 1) * s
+    return True
+
+
 def _nested(t):
     """(stride, size) of t's dimensions of more than one element, innermost first, and whether no two elements share an address
     (every stride steps over what the dimensions inside it span)."""
     dims = sorted([(s, n) for n, s in zip(t.shape, t.stride()) if n > 1])
-    span = 1
-    for s, n in dims:
-        if s < span:
-            return dims, False
-        span += (n - 1) * s
-    return dims, True
+    return dims, _nest(dims, 1)
 
 
 def writable(t):
@@ -201,10 +205,10 @@ def disjoint(a, b):
     da, db = _nested(a)[0], _nested(b)[0]
     if gap > sum([(n - 1) * s for s, n in da]):
         return True
-    for k in range(len(da)):  # the k innermost dimensions of a against what the next one leaves for b
+    for k in range(len(da)):  # the k innermost dimensions of a against what the next one leaves for b (if the outer ones step over all of that)
         outer = da[k:]
         m = len(db) - len(outer)
-        if m < 0 or db[m:] != outer:
+        if m < 0 or db[m:] != outer or not _nest(outer, outer[0][0]):
             continue
         span_a, span_b = 1 + sum([(n - 1) * s for s, n in da[:k]]), 1 + sum([(n - 1) * s for s, n in db[:m]])
         if gap >= span_a and gap + span_b <= outer[0][0]:

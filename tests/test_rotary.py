@@ -242,6 +242,24 @@ def test_views_that_share_memory():
     assert not _lib.writable(torch.zeros(20).as_strided((3, 8), (4, 1))) and _lib.same_view(q, qkv[:, :, 0]) and not _lib.same_view(q, k)
 
 
+def test_views_called_disjoint_or_writable_are():
+    """Against a count of every element's address; overlapping outer dimensions among them."""
+    buf, said = torch.zeros(4000), 0
+    for B, N, H, Hk, D in ((1, 2, 1, 1, 4), (2, 3, 2, 1, 4), (2, 1, 2, 2, 4), (3, 2, 1, 2, 6)):
+        for sn in (4, 8, 12, 16, 24, 30):
+            for sb in (4, 12, N * sn, N * sn + 4, 2 * sn, sn):
+                for sh, th in ((4, 4), (6, 4), (3, 6), (12, 12)):
+                    for q0, k0 in ((0, 4), (0, 8), (8, 0), (0, 12), (12, 0), (16, 4), (0, 500)):
+                        q, k = buf.as_strided((B, N, H, D), (sb, sn, sh, 1), q0), buf.as_strided((B, N, Hk, D), (sb, sn, th, 1), k0)
+                        at = [[t.storage_offset() + sum(i * s for i, s in zip(index, t.stride()))
+                               for index in torch.cartesian_prod(*map(torch.arange, t.shape)).tolist()] for t in (q, k)]
+                        for t, own in zip((q, k), at):
+                            assert not _lib.writable(t) or len(set(own)) == len(own), (t.shape, t.stride())
+                        assert not _lib.disjoint(q, k) or not set(at[0]) & set(at[1]), (q.shape, q.stride(), k.shape, k.stride(), q0, k0)
+                        said += _lib.disjoint(q, k) and k0 != 500
+    assert said > 100
+
+
 def test_entry_point_refusals():
     import ctypes
     lib, A = _lib.load(), 0x7F0000000000
