@@ -133,8 +133,22 @@ def rotary(q, k, positions, plan, n_prefix=0, inverse=False, out=None):
     return result
 
 
+def _side_by_side(q, k):
+    """Whether q and k surely are, as in a packed projection, parts of rows of one buffer that share no element with each other or
+    among themselves (the general checks say the same of more views, and take 10 us for it)."""
+    B, N, H, D = q.shape
+    sb, sn, sh, _ = q.stride()
+    tb, tn, th, _ = k.stride()
+    if sn != tn or sb != tb or N < 2 or (B > 1 and sb < N * sn) or sh < D or th < D:
+        return False
+    gap, q_row, k_row = (k.data_ptr() - q.data_ptr()) // q.element_size(), (H - 1) * sh + D, (k.shape[2] - 1) * th + D
+    return gap >= q_row and gap + k_row <= sn or -gap >= k_row and q_row - gap <= sn
+
+
 def _checked(out, q, k):
     """The caller's pair of outputs, refused where two threads could meet on an element."""
+    if k is not None and len(out) == 2 and out[0] is q and out[1] is k and _side_by_side(q, k):
+        return q, k
     inputs, outs = [q] if k is None else [q, k], list(out)
     if len(outs) == 2 and k is None and outs[1] is None:
         outs.pop()

@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from fastbb_b200 import _lib
-from fastbb_b200.rotary import RotaryPlan, axial_plan, grid_positions, rotary, rotary_plan
+from fastbb_b200.rotary import RotaryPlan, _checked, _side_by_side, axial_plan, grid_positions, rotary, rotary_plan
 
 
 def reference(x, positions, plan, n_prefix, inverse):
@@ -244,7 +244,7 @@ def test_views_that_share_memory():
 
 def test_views_called_disjoint_or_writable_are():
     """Against a count of every element's address; overlapping outer dimensions among them."""
-    buf, said = torch.zeros(4000), 0
+    buf, said, quick = torch.zeros(4000), 0, 0
     for B, N, H, Hk, D in ((1, 2, 1, 1, 4), (2, 3, 2, 1, 4), (2, 1, 2, 2, 4), (3, 2, 1, 2, 6)):
         for sn in (4, 8, 12, 16, 24, 30):
             for sb in (4, 12, N * sn, N * sn + 4, 2 * sn, sn):
@@ -257,7 +257,13 @@ def test_views_called_disjoint_or_writable_are():
                             assert not _lib.writable(t) or len(set(own)) == len(own), (t.shape, t.stride())
                         assert not _lib.disjoint(q, k) or not set(at[0]) & set(at[1]), (q.shape, q.stride(), k.shape, k.stride(), q0, k0)
                         said += _lib.disjoint(q, k) and k0 != 500
-    assert said > 100
+                        if _side_by_side(q, k):
+                            assert _lib.writable(q) and _lib.writable(k) and not set(at[0]) & set(at[1]), (q.shape, q.stride(), k.shape, k.stride(), q0, k0)
+                            assert all(a is b for a, b in zip(_checked((q, k), q, k), (q, k)))
+                            quick += 1
+    assert said > quick > 20
+    q, k, _ = torch.zeros(2, 5, 3, 4, 8).unbind(2)
+    assert _side_by_side(q, k) and _side_by_side(k, q) and not _side_by_side(q, q)
 
 
 def test_entry_point_refusals():
