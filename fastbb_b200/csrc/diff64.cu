@@ -314,19 +314,19 @@ diff64_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
                 return true;
             };
             uint32_t g = 0;
-            int n = 0, nq = 0;  // items, and those with keys
+            int n = 0;  // items with keys; of others no barrier hears anything
             bool ok = true;
 #pragma unroll 1
-            for (; it.more(a) && ok; it.next(a), ++n) {
+            for (; it.more(a) && ok; it.next(a)) {
                 const int here = it.here, halves = (here + 63) / 64;
-                if (here > 0) {
-                    ok = all_ok(mbar_wait(q_full, (uint32_t)nq & 1u, s_abort, DEV_TIMEOUT_TMA_FULL, 100));
-                    ++nq;
-                    ok = ok && scores(g, 0, halves == 1);
-                    if (ok && halves > 1) ok = scores(g + 1u, 1, halves == 2);
-                }
-                // the softmax warps have read the last item's O (every item's phase is waited for: none may be skipped)
+                if (here <= 0) continue;
+                ok = all_ok(mbar_wait(q_full, (uint32_t)n & 1u, s_abort, DEV_TIMEOUT_TMA_FULL, 100));
+                ok = ok && scores(g, 0, halves == 1);
+                if (ok && halves > 1) ok = scores(g + 1u, 1, halves == 2);
+                // the softmax warps have read the last such item's O. No phase of theirs is missed here: the next one needs this item's
+                // products of both maps, which come behind this wait.
                 if (ok && n > 0) ok = all_ok(mbar_wait(o_free, (uint32_t)(n - 1) & 1u, s_abort, DEV_TIMEOUT_TMEM_EMPTY, 40 + t));
+                ++n;
 #pragma unroll 1
                 for (int i = 0; i < halves && ok; ++i, ++g) {
                     if ((i & 1) == 0 && !all_ok(mbar_wait(v_full(vs), vph, s_abort, DEV_TIMEOUT_TMA_FULL, 16 + vs))) { ok = false; break; }
@@ -378,15 +378,18 @@ diff64_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
             ok = mbar_wait(meeting(u), met & 1u, s_abort, DEV_TIMEOUT_OTHER, 230 + u) && ok;
             ++met;
         };
-        // an item's end: O has been read (an earlier item's phase must be complete before this one's arrivals begin)
+        // the end of an item with keys: O has been read (an earlier one's phase must be complete before this one's arrivals begin). Items
+        // without keys have no part in it: nothing would hold these warps back there, and a phase that completes before an issuer has
+        // looked for the one ahead of it takes that one from its sight.
         auto release = [&]() {
             tc_fence_before();
             ok = (n == 0 || mbar_wait(o_free, (uint32_t)(n - 1) & 1u, s_abort, DEV_TIMEOUT_OTHER, 44)) && ok;
             __syncwarp();
             if (lane == 0) mbar_arrive(o_free);
+            ++n;
         };
 #pragma unroll 1
-        for (; it.more(a) && ok; it.next(a), ++n) {
+        for (; it.more(a) && ok; it.next(a)) {
             const int here = it.here, halves = (here + 63) / 64;
             const int row0 = it.qt * FQ + lane_base, rowA = row0 + (lane >> 2), rowB = rowA + 8;
             if (row0 >= a.Nq) {
@@ -399,7 +402,7 @@ diff64_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
                     __syncwarp();
                     if (ok && lane == 0) mbar_arrive(p_ready(t, g & 1u));
                 }
-                release();
+                if (halves > 0) release();
                 continue;
             }
             const bool whole = a.splits == 1;
@@ -498,8 +501,8 @@ diff64_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
                     float2* stat = reinterpret_cast<float2*>(dst + 16 * 128);
                     if (cq == 0) stat[lane >> 2] = make_float2(mA, lA);
                     if (cq == 1) stat[(lane >> 2) + 8] = make_float2(mB, lB);
+                    release();
                 }
-                release();
                 continue;
             }
             // Columns 64 t .. 64 t + 63 of the tile's rows: o = O_1 / l_1 - lam O_2 / l_2. The other map's warp of these rows has waited for
@@ -526,11 +529,11 @@ diff64_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
 #pragma unroll
                     for (int i = 0; i < 8; ++i) o[8 * c + i] = __uint_as_float(x[i]) * ((i & 2) ? f1B : f1A) - __uint_as_float(y[i]) * ((i & 2) ? f2B : f2A);
                 }
+                release();
             } else {
 #pragma unroll
                 for (int i = 0; i < 32; ++i) o[i] = 0.f;
             }
-            release();
             float scA = a.out_scale, scB = a.out_scale;
             const bool norm = a.weight != nullptr && halves > 0;
             if (norm) {

@@ -114,6 +114,38 @@ def test_many_tiles_of_uneven_lengths(B, Nq, Nk, H):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("B", [32, 40])
+@pytest.mark.parametrize("keyed", ["first", "middle", "last", "both ends", "every seventh", "one in all"])
+def test_long_runs_of_entries_without_keys(B, keyed):
+    """Every CTA has many tiles in a row without keys, ahead of, between and behind those with some; in falling order of the lengths (32 entries) and in
+    the entries' own (40). Rows beyond the queries' in every last tile."""
+    g = torch.Generator("cuda").manual_seed(B)
+    Nq, Nk, H = 1000, 130, 8
+    q, k, v, lam = make(B, Nq, Nk, H, H // 2, g, "token")
+    which = {"first": range(2), "middle": range(B // 2, B // 2 + 2), "last": range(B - 2, B), "both ends": (0, B - 1), "every seventh": range(0, B, 7),
+             "one in all": (B // 3,)}[keyed]
+    lengths = [(1, 64, 65, 130, 128, 17)[i % 6] if i in which else -(i % 2) for i in range(B)]
+    weight = torch.randn(128, generator=g, device="cuda").half()
+    n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    for _ in range(3):
+        out = diff_attention(q, k, v, lam, weight=weight, key_lengths=n)
+    rest = torch.tensor([m <= 0 for m in lengths], device="cuda")
+    assert bool((out[rest] == 0).all())
+    check(out[~rest], q[~rest], k[~rest], v[~rest], lam[~rest], weight=weight, lengths=[m for m in lengths if m > 0])
+    assert _lib.device_status() == (0, 0, 0, 0)
+
+
+@pytest.mark.gpu
+def test_thousands_of_tiles_without_keys():
+    g = torch.Generator("cuda").manual_seed(1)
+    q, k, v, lam = make(16, 2900, 0, 8, 8, g)
+    out = torch.full((16, 2900, 8, 128), float("nan"), device="cuda", dtype=torch.float16)
+    for _ in range(3):
+        assert bool((diff_attention(q, k, v, lam, weight=torch.ones(128, device="cuda"), out=out) == 0).all())
+    assert _lib.device_status() == (0, 0, 0, 0)
+
+
+@pytest.mark.gpu
 def test_no_keys_at_all():
     g = torch.Generator("cuda").manual_seed(1)
     q, k, v, lam = make(2, 5, 0, 2, 2, g)
