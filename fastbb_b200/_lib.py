@@ -216,6 +216,26 @@ def disjoint(a, b):
     return False
 
 
+def apart(out, *others):
+    """Whether an output surely shares no memory with any of the others (of any dtype; None: not there)."""
+    lo = out.data_ptr()
+    hi = lo + _bytes(out)
+    for t in others:
+        if t is not None:
+            p = t.data_ptr()
+            if p < hi and lo < p + _bytes(t) and not (t.dtype == out.dtype and disjoint(out, t)):
+                return False
+    return True
+
+
+def _bytes(t):
+    """From a tensor's first byte to behind its last one, holes included."""
+    n = t.numel()
+    if n and not t.is_contiguous():
+        n = 1 + sum([(n - 1) * s for n, s in zip(t.shape, t.stride())])
+    return n * t.element_size()
+
+
 def device_status():
     """Synchronise the current device and raise FastbbError if any kernel gave up a bounded wait."""
     out = (ctypes.c_uint * 4)()

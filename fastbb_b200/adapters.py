@@ -48,7 +48,7 @@ def adapter_linear(x, w, adapters, ids, offsets=None, b=None, act=None, res=None
     ids: int32 [S] on the GPU, the adapter of each request; a number out of [0, L) (say -1): none.
     offsets: int32 [S + 1] on the GPU, not decreasing: request s has rows offsets[s] .. offsets[s + 1] - 1 of x's rows taken in order; rows of
     no request have no adapter. Without offsets x's first dimension is the requests, [S, ..., K].
-    out: fp16 and contiguous, may be res itself, shares no memory with x."""
+    out: fp16 and contiguous, may be res itself, shares no memory with any other input."""
     if act not in _ACT:
         raise ValueError(f"unsupported activation: {act}")
     device = x.device
@@ -81,7 +81,8 @@ def adapter_linear(x, w, adapters, ids, offsets=None, b=None, act=None, res=None
     else:
         if out.shape != oshape or out.device != device or out.dtype != torch.float16 or not out.is_contiguous() or out.data_ptr() % 16:
             raise ValueError("out must be contiguous with the output shape, input dtype and device")
-        if not (_lib.disjoint(out, x) and _lib.disjoint(out, w) and (res is None or _lib.same_view(out, res) or _lib.disjoint(out, res))):
+        if not (_lib.apart(out, x, w, b, gamma, adapters.down, adapters.up, adapters.scale, ids, offsets) and (
+                res is None or _lib.same_view(out, res) or _lib.disjoint(out, res))):
             raise ValueError("out may be res itself and shares no memory with the other inputs")
     if x.is_contiguous():
         x2, lda = x, K

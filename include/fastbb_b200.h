@@ -195,7 +195,7 @@ int fbb_flash64_f16_static(const void* q, const void* k, const void* v, void* o,
 /* ---- a linear layer with the low-rank adapters of many requests ---------------------------------------------------------------
  * C = epilogue(A . W^T + scale_a (A . down_a^T) . up_a^T), a the adapter of the row's request: one shared projection for fine-tuned variants
  * of a model served together. The layer itself is fbb_linear_f16's (same arguments, epilogues and requirements; fp32 accumulator); C may
- * share memory with res (same pointer and stride) but not with A. No counterpart in the reference.
+ * share memory with res (same pointer and stride) but with no other input (A is checked for). No counterpart in the reference.
  * down: [adapters, rank, K], up: [adapters, N, rank], fp16, contiguous, 16-byte aligned; scale: [adapters] fp32. rank: a multiple of 8 up to
  * 128 (smaller ones are padded with zeros by the caller). ids: int32 [requests], an id out of [0, adapters) means no adapter.
  * offsets: int32 [requests + 1], not decreasing: request s has rows offsets[s] .. offsets[s + 1] - 1; rows of no request have no adapter. null:

@@ -243,6 +243,30 @@ def test_refusals_on_the_gpu():
         adapter_linear(x3, w, slots, ids, act="swiglu", res=torch.zeros(3, 4, 64, device="cuda").half())
 
 
+@pytest.mark.gpu
+def test_outputs_over_any_input_are_refused():
+    """out shares its first bytes, or its last, with one input at a time; right behind it or ahead of it the call is taken."""
+    g = torch.Generator("cuda").manual_seed(11)
+    x, w, slots, b = make(16, 64, 128, 8, 2, g)
+    ids, bounds, res, gamma = vector([0, 1, -1]), vector([0, 4, 12, 16]), torch.zeros(16, 128, device="cuda").half(), b.clone()
+    size = 2 * 16 * 128
+    store = torch.zeros(1 << 17, dtype=torch.uint8, device="cuda")
+    parts = dict(x=x, w=w, b=b, gamma=gamma, down=slots.down, up=slots.up, scale=slots.scale, ids=ids, offsets=bounds, res=res)
+    for name, t in parts.items():
+        n, base = t.numel() * t.element_size(), 1 << 16
+        for clear, shared in ((base + (n + 15) // 16 * 16, base + (n + 15) // 16 * 16 - 16), (base - size, base - size + 16)):
+            view = store[base:base + n].view(t.dtype).view(t.shape)
+            view.copy_(t)
+            use = {**parts, name: view}
+            call = lambda lo: adapter_linear(use["x"], use["w"], Adapters(use["down"], use["up"], use["scale"]), use["ids"], use["offsets"], b=use["b"],  # noqa: E731, B023
+                                             res=use["res"], gamma=use["gamma"], out=store[lo:lo + size].view(torch.float16).view(16, 128))
+            held = store.clone()
+            with pytest.raises(ValueError, match="shares no memory"):
+                call(shared)
+            assert torch.equal(store, held)
+            call(clear)
+
+
 # ------------------------------------------------------------------------------------------------------------------ CPU
 def test_cpu_tensors_are_refused():
     with pytest.raises(ValueError, match="no CPU path"):
