@@ -32,7 +32,7 @@ def diff_attention(q, k, v, lam, weight=None, eps=1e-5, out_scale=1.0, scale=Non
     out_scale: a factor of the result, with or without the norm. scale: of the scores, 64^-0.5 unless given, > 0
     (scaled scores may reach 6e7 in magnitude).
     key_lengths: int32 [B] on the GPU: keys from key_lengths[b] on are not seen, whatever they hold; a row without keys is 0.
-    out: fp16 [B, Nq, H, 128] that shares no memory with the inputs."""
+    out: fp16 [B, Nq, H, 128] that shares no memory with any input."""
     uq, uk, uv = _usable(q, 64), _usable(k, 64), _usable(v, 128)
     if uq is None or uk is None or uv is None:
         raise ValueError("diff_attention needs CUDA fp16 q, k [B, N, 2 * heads, 64] and v [B, N, heads, 128] with a contiguous last dim, other strides "
@@ -66,7 +66,7 @@ def diff_attention(q, k, v, lam, weight=None, eps=1e-5, out_scale=1.0, scale=Non
     elif not (_usable(out, 128) is not None and out.shape == (B, Nq, H, 128) and out.device == device and _lib.writable(out)):
         raise ValueError("out must be fp16 [B, Nq, H, 128] on the inputs' device, with a contiguous last dim, strides that are multiples of 8 elements, "
                          "16-byte aligned and no element twice")
-    elif not (_lib.disjoint(out, q) and _lib.disjoint(out, k) and _lib.disjoint(out, v)):
+    elif not _lib.apart(out, q, k, v, lam, weight, key_lengths):
         raise ValueError("out shares memory with an input")
     if B == 0 or Nq == 0:
         return out

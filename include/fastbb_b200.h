@@ -228,7 +228,7 @@ int fbb_adapter_linear_f16_from(const fbb_adapter_linear_args* args);
  * in the reference; it stands beside fbb_flash64_f16, with one launch (and one pass over v) for what takes four of that.
  * q: [B, Nq, 2H, 64], head h's maps are heads 2h and 2h + 1; k: [B, Nk, 2Hk, 64]; v: [B, Nk, Hk, 128]; o: [B, Nq, H, 128]; fp16, last
  * dimension contiguous, the other strides (batch, token, head) multiples of 8 elements, positive where the dimension has more than one
- * element; Hk divides H (query heads in a row share a key head). lam: fp32 [B, Nq, H] with strides of its own (0: broadcast).
+ * element; Hk divides H (query heads in a row share a key head). o shares no memory with any input. lam: fp32 [B, Nq, H] with strides of its own (0: broadcast).
  * weight: [128] of weight_dtype (fp16 or fp32) or null. lengths: int32 [B] or null; keys from lengths[b] on are not seen, whatever k and
  * v hold there (a number below 0 counts as 0, beyond Nk as Nk); without any key a row of o is 0. scale > 0.
  * Scores, maxima, sums and outputs are fp32; the probabilities are rounded to fp16 for the second product, relative to a maximum that

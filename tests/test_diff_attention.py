@@ -290,6 +290,28 @@ def test_refusals_on_the_gpu():
             call()
 
 
+@pytest.mark.gpu
+def test_outputs_over_any_input_are_refused():
+    """out shares 16 bytes with one input at a time; right behind it the call is taken."""
+    g = torch.Generator("cuda").manual_seed(8)
+    q, k, v, lam = make(2, 20, 30, 2, 1, g, "token")
+    parts = dict(q=q, k=k, v=v, lam=lam, weight=torch.ones(128, device="cuda"), lengths=torch.tensor([30, 7], dtype=torch.int32, device="cuda"))
+    size = 2 * q.numel() // 64 * 64
+    store = torch.zeros(1 << 18, dtype=torch.uint8, device="cuda")
+    for name, t in parts.items():
+        n = t.numel() * t.element_size()
+        view = store[:n].view(t.dtype).view(t.shape)
+        view.copy_(t)
+        use = {**parts, name: view}
+        call = lambda lo: diff_attention(use["q"], use["k"], use["v"], use["lam"], weight=use["weight"], key_lengths=use["lengths"],  # noqa: E731, B023
+                                         out=store[lo:lo + size].view(torch.float16).view(2, 20, 2, 128))
+        clear, held = (n + 15) // 16 * 16, store.clone()
+        with pytest.raises(ValueError, match="shares memory"):
+            call(clear - 16)
+        assert torch.equal(store, held)
+        call(clear)
+
+
 # ------------------------------------------------------------------------------------------------------------------ CPU
 def test_cpu_tensors_are_refused():
     q = torch.zeros(1, 4, 2, 64).half()
