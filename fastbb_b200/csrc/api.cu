@@ -379,6 +379,17 @@ int fbb_rotary(const fbb_rotary_tensor* tensors, int n_tensors, int B, int N, in
         if (positions == nullptr) return fail(FBB_ERR_NULL, "rotary: positions is null");
         if (reinterpret_cast<uintptr_t>(positions) & (pos_dtype == FBB_POS_I64 ? 7u : 3u)) return fail(FBB_ERR_ALIGN, "rotary: positions must be aligned to their elements");
     }
+    // what every thread reads while others write y: the positions, from the first to the last, and the plan
+    struct Bytes { uintptr_t lo, hi; };
+    auto bytes = [](const void* p, int64_t elements, int64_t size) { return Bytes{reinterpret_cast<uintptr_t>(p), reinterpret_cast<uintptr_t>(p) + (uintptr_t)(elements * size)}; };
+    const Bytes read[3] = {bytes(positions, N > n_prefix ? (B - 1) * p_sb + (N - n_prefix - 1) * p_sn + (n_axes - 1) * p_sa + 1 : 0, pos_dtype == FBB_POS_I64 ? 8 : 4),
+                           bytes(freqs, pairs, 4), bytes(axes, pairs, 4)};
+    for (int i = 0; i < n_tensors; ++i) {
+        const fbb_rotary_tensor& t = tensors[i];
+        const Bytes y = bytes(t.y, (B - 1) * t.y_sb + (N - 1) * t.y_sn + (t.heads - 1) * t.y_sh + D, dtype == FBB_DTYPE_F32 ? 4 : 2);
+        for (const Bytes& r : read)
+            if (r.lo < y.hi && y.lo < r.hi) return fail(FBB_ERR_SHAPE, "rotary: y of tensor %d shares memory with the positions, freqs or axes", i);
+    }
     return launch_rotary(tensors, n_tensors, B, N, D, pairs, pairing, n_prefix, positions, pos_dtype, n_axes, p_sb, p_sn, p_sa, freqs, axes, inverse,
                          dtype, (cudaStream_t)stream);
 }

@@ -80,7 +80,8 @@ def rotary(q, k, positions, plan, n_prefix=0, inverse=False, out=None):
 
     positions: [N - n_prefix, axes] for every sequence alike, or [B, N - n_prefix, axes]; int32, int64 or fp32.
     inverse: the transposed rotation, which undoes this one and takes gradients of (q', k') to gradients of (q, k).
-    out: (q_out, k_out); each may be its own input (in place), otherwise it shares no memory with either input."""
+    out: (q_out, k_out); each may be its own input (in place), otherwise it shares no memory with any input.
+    Positions and plan lie outside it altogether, not in the gaps of a strided one."""
     shape, device, dtype = q.shape, q.device, q.dtype
     code = _lib.DTYPE_CODE.get(dtype)
     if not q.is_cuda or code is None or len(shape) != 4:

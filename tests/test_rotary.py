@@ -194,6 +194,22 @@ def test_refusals_on_the_gpu():
 
 
 @pytest.mark.gpu
+def test_outputs_over_the_positions_or_the_plan_are_refused():
+    store = torch.zeros(4096, device="cuda")
+    q, where = store[:1024].view(1, 8, 2, 64), store[1000:1016].view(8, 2)
+    plan = axial_plan(64)
+    held = store.clone()
+    with pytest.raises(_lib.FastbbError, match="shares memory"):
+        rotary(q, None, where, plan, out=(q, None))
+    with pytest.raises(_lib.FastbbError, match="shares memory"):
+        rotary(torch.zeros_like(q), q, where, plan, out=(torch.zeros_like(q), q))
+    with pytest.raises(_lib.FastbbError, match="shares memory"):
+        rotary(q, None, store[2000:2016].view(8, 2), RotaryPlan(store[64:96], plan.axes, 2, "half"), out=(q, None))
+    assert torch.equal(store, held)
+    rotary(q, None, store[1024:1040].view(8, 2), plan, out=(q, None))  # beside it is well
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("B,N", [(1, 2 ** 31), (1, 2 ** 32 + 1), (2 ** 16, 2 ** 15), (2 ** 32 + 1, 1)])
 def test_more_tokens_than_31_bits_count_are_refused(B, N):
     """(Views of a single row: nothing is allocated.)"""
@@ -264,6 +280,37 @@ def test_views_called_disjoint_or_writable_are():
     assert said > quick > 20
     q, k, _ = torch.zeros(2, 5, 3, 4, 8).unbind(2)
     assert _side_by_side(q, k) and _side_by_side(k, q) and not _side_by_side(q, q)
+
+
+def test_outputs_apart_from_inputs_of_any_type():
+    store = torch.zeros(4096, dtype=torch.uint8)
+    out = store[1024:2048].view(torch.float16).view(4, 2, 64)
+    for dtype in (torch.float32, torch.int32, torch.int64, torch.float16):
+        inside = lambda lo, hi: store[lo:hi].view(dtype)  # noqa: E731, B023
+        assert _lib.apart(out, None, inside(0, 1024), inside(2048, 4096), inside(1024, 1024), torch.zeros(9, dtype=dtype))
+        for lo, hi in ((1016, 1032), (1024, 1032), (2040, 2048), (2040, 4096), (0, 4096), (1500 // 8 * 8, 1600)):
+            assert not _lib.apart(out, None, inside(0, 1024), inside(lo, hi))
+        assert not _lib.apart(out, inside(0, 4096)[::4096 // dtype.itemsize - 1])                                  # the holes of another type's view count
+        assert not _lib.apart(store[:2048].view(torch.float16).view(8, 128)[:, :8], store[20:24].view(torch.int32)) and _lib.apart(out[:0], inside(0, 4096))
+    assert _lib.apart(out[..., :32], out[..., 32:]) and not _lib.apart(out[..., :32], out[..., 31:])             # views of its own type: the elements
+
+
+def test_entry_point_refuses_outputs_over_the_positions_or_the_plan():
+    lib, y = _lib.load(), 0x7F0000000000
+    # y: [2, 5, 3, 64] fp32 in slots of 256, 2 x 5 x 4 of them but the last
+    last = y + 4 * ((1 * 5 + 4) * 1024 + 2 * 256 + 64)
+
+    def call(pos=y - 4096, freqs=y - 8192, ax=y - 16384, second=False, pd=2, p=(8, 2, 1), B=2):
+        tensor, other = (y, y, 3, *(5120, 1024, 256) * 2), (y - (1 << 20), y - (1 << 20), 3, *(5120, 1024, 256) * 2)
+        first, second = (other, tensor) if second else (tensor, other)
+        status = lib.fbb_rotary_from(_lib.RotaryArgs.pack(*first, *second, pos, freqs, ax, 0, *p, 2, B, 5, 64, 32, 0, 1, pd, 2, 0, 2))
+        return status, b"shares memory" in lib.fbb_last_error()
+
+    for second in (False, True):
+        for at in (y, last - 4, y + 4096, y + 300):
+            assert call(pos=at, second=second) == call(freqs=at, second=second) == call(ax=at, second=second) == (-2, True)
+        assert call(freqs=y - 4 * 31, second=second) == call(ax=y - 4 * 31, second=second) == (-2, True)
+        assert call(pos=y - 4 * (8 + 3 * 2 + 1), second=second) == call(pos=y - 8 * (8 + 3 * 2 + 1), pd=1, second=second) == (-2, True)
 
 
 def test_entry_point_refusals():
