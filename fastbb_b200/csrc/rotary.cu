@@ -7,9 +7,11 @@
 // measured copy rate, 12.2 measured; fp32 at 4 x 1374 tokens x 48 x 64: 20.6 and 24.5). The angles of a token are the same for all its
 // heads, so a CTA takes a few whole tokens, works their cos / sin out once into shared memory, and streams the tokens' heads through with
 // 16-byte accesses, kRotaryUnroll items in flight per thread (2 and 8 were slower: 54 - 66 and 53 us on 2 x 8184 x 20 x 128 bf16, now 37).
-// The angle is a product in 64 bits (an integer position times an fp32 frequency, exact up to 2^29; far positions lose nothing),
-// reduced to a fraction of a turn there; sincospif of twice that, at most 1, then has fp32 accuracy at any position. The products and
-// the sum are fp32, rounded once to the output type.
+// The angle, position times fp32 frequency, and its number of turns are doubles up to 2^20 radians, off by 2^-31 radians at most. Beyond, each is
+// a double and the remainder that its rounding left (Dekker's arithmetic: a product's remainder is one fma; 1 / (2 pi) is two doubles as
+// well), off by 2^-105 of the number of turns: fp32 angles lose nothing up to position times frequency of 2^70, which every int64 position
+// is within for frequencies up to 2^7. (All angles that way: 3 % more on the fp32 case below.) The turns' fraction is taken there;
+// sincospif of twice that, at most 1, then has fp32 accuracy. The products and the sum are fp32, rounded once to the output type.
 #include <cuda_bf16.h>
 
 #include "common.cuh"
@@ -46,6 +48,26 @@ __device__ __forceinline__ double rotary_position(const RotaryArgs& a, int64_t a
     if (a.pos_dtype == FBB_POS_I32) return (double)reinterpret_cast<const int*>(a.pos)[at];
     if (a.pos_dtype == FBB_POS_I64) return (double)reinterpret_cast<const int64_t*>(a.pos)[at];
     return (double)reinterpret_cast<const float*>(a.pos)[at];
+}
+// The fraction of a turn, from -1/2 to 1/2, of the position at `at` times freq radians.
+__device__ __forceinline__ double rotary_fraction(const RotaryArgs& a, int64_t at, double freq) {
+    constexpr double kTurn = 0x1.45f306dc9c883p-3, kTurnRest = -0x1.6b01ec5417056p-57;  // their sum is 1 / (2 pi) to 2^-108 of it
+    double position = rotary_position(a, at), angle = position * freq, turns = angle * kTurn, fraction = turns - rint(turns);
+    if (fabs(angle) >= 1048576.0) {
+        double angle_rest = 0.0;
+        if (a.pos_dtype == FBB_POS_I64) {
+            const int64_t p = reinterpret_cast<const int64_t*>(a.pos)[at];
+            const double high = (double)(p >> 32) * 4294967296.0, low = (double)(uint32_t)p;  // (both exact)
+            position = high + low;
+            angle_rest = (low - (position - high)) * freq;
+        }
+        angle = position * freq;
+        angle_rest += fma(position, freq, -angle);
+        turns = angle * kTurn;
+        fraction = (turns - rint(turns)) + (fma(angle, kTurn, -turns) + fma(angle, kTurnRest, angle_rest * kTurn));
+        fraction -= rint(fraction);
+    }
+    return fraction;
 }
 
 template <typename T>
@@ -101,8 +123,10 @@ struct RotaryRow {
 // HALF: pairing. VEC: 16-byte accesses; the scalar form (columns one by one) takes every size and stride that is not a multiple of
 // 16 bytes. A vector item of the half pairing is the two vectors at columns 8c and P + 8c, of the other pairing one vector; what is
 // left of a head (columns from 2P on) are plain copies behind them.
+// (Three or four CTAs an SM: left to itself the code for far angles takes 88 registers of the half pairing's vector form, 73 of the
+// other's, and a CTA from each SM: 13.7 instead of 12.1 us on 6145 tokens, 42.7 instead of 37.3 on 2 x 8184 x 20 x 128.)
 template <typename T, bool HALF, bool VEC>
-__global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryArgs a) {
+__global__ void __launch_bounds__(kRotaryThreads, HALF && VEC ? 3 : 4) rotary_kernel(const RotaryArgs a) {
     __shared__ __align__(16) float2 s_turn[kRotaryTableEntries];
     __shared__ RotaryRow s_row[kRotaryMaxTokens];
     __shared__ int s_pass[kRotaryMaxTokens];  // a row without a position
@@ -215,8 +239,7 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryArgs
         float2 turn = make_float2(1.f, 0.f);
         if (n >= 0) {
             const int axis = min(max(a.axes[p], 0), a.n_axes - 1);
-            const double turns = rotary_position(a, (int64_t)b * a.p_sb + n * a.p_sn + axis * a.p_sa) * (double)a.freqs[p] * 0.15915494309189533577;
-            sincospif(2.f * (float)(turns - rint(turns)), &turn.y, &turn.x);
+            sincospif(2.f * (float)rotary_fraction(a, (int64_t)b * a.p_sb + n * a.p_sn + axis * a.p_sa, (double)a.freqs[p]), &turn.y, &turn.x);
             turn.y *= a.sign;
         }
         s_turn[i] = turn;

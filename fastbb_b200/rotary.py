@@ -78,7 +78,8 @@ def rotary(q, k, positions, plan, n_prefix=0, inverse=False, out=None):
     """(q', k'): q [B, N, H, D] and k [B, N, Hk, D] (fp16, bf16 or fp32, D contiguous, any other strides; k may be None) turned by the
     positions of their tokens. Columns from 2 * pairs on, and the first n_prefix rows of every sequence, pass unchanged.
 
-    positions: [N - n_prefix, axes] for every sequence alike, or [B, N - n_prefix, axes]; int32, int64 or fp32.
+    positions: [N - n_prefix, axes] for every sequence alike, or [B, N - n_prefix, axes]; int32, int64 or fp32. Angles keep fp32 accuracy
+    up to position * frequency of 2^70.
     inverse: the transposed rotation, which undoes this one and takes gradients of (q', k') to gradients of (q, k).
     out: (q_out, k_out); each may be its own input (in place), otherwise it shares no memory with any input.
     Positions and plan lie outside it altogether, not in the gaps of a strided one."""

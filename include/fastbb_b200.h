@@ -262,7 +262,7 @@ int fbb_diff64_f16_from(const fbb_diff64_args* args);
  * Pair i < pairs of every head's D columns, in a row whose position on axis axes[i] is p, is turned by t = p * freqs[i]:
  *   (x, y) -> (x cos t - y sin t, y cos t + x sin t), or by -t with inverse != 0 (the transposed rotation: the gradient's).
  * FBB_ROTARY_HALF: a pair is columns (i, i + pairs); FBB_ROTARY_PAIRS: columns (2i, 2i + 1). Columns from 2 * pairs on and the
- * first n_prefix rows of every sequence pass unchanged. Angles are products in 64 bits, reduced before sine and cosine in 32;
+ * first n_prefix rows of every sequence pass unchanged. Angles are reduced to a turn in two doubles ahead of sine and cosine in fp32;
  * the rotation is fp32, rounded once.
  * tensors: one or two of {x, y, heads, strides of [B, N, heads, D] in elements, D contiguous}; y may be x itself, otherwise it
  * shares no memory with any x; positions, freqs and axes lie outside it, gaps of its strides included (refused otherwise). positions: [B, N - n_prefix, n_axes] of pos_dtype with strides p_sb, p_sn, p_sa (p_sb 0: the same

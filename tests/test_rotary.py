@@ -5,6 +5,7 @@ cosine are off by up to 2 steps (2^-23), the two products and their sum by one r
 less than (|x| + |y|) 2^-21. The result is rounded to its type once: half a step of it, eps / 2 relative, or half of the smallest
 subnormal."""
 import math
+from fractions import Fraction
 
 import pytest
 import torch
@@ -93,6 +94,47 @@ def test_far_positions_of_every_type(dtype):
     assert torch.equal(rotary(q, None, strided, plan)[0], rotary(q, None, where, plan)[0])
     columns = where.t().contiguous().t()
     assert torch.equal(rotary(q, None, columns, plan)[0], rotary(q, None, where, plan)[0])
+
+
+def fractions_of_a_turn(positions, freqs):
+    """position * freq / (2 pi) without its whole turns, from integers of 400 bits (pi by Machin's formula)."""
+    def arctan_of_inverse(n, bits=400):
+        term, total, k, sign = (1 << bits) // n, 0, 1, 1
+        while term:
+            total, term, k, sign = total + sign * (term // k), term // (n * n), k + 2, -sign
+        return total
+    turn = Fraction(2 * 4 * (4 * arctan_of_inverse(5) - arctan_of_inverse(239)), 1 << 400)
+    turns = [[Fraction(p) * Fraction(f) / turn for f in freqs] for p in positions]
+    return torch.tensor([[float(t - round(t)) for t in row] for row in turns], dtype=torch.float64)
+
+
+def test_the_exact_fractions_are():
+    got = fractions_of_a_turn([0, 1, -7, 3.5], [1.0, 0.25]) * 2 * math.pi
+    for row, p in zip(got.tolist(), (0, 1, -7, 3.5)):
+        for angle, f in zip(row, (1.0, 0.25)):
+            assert math.isclose(math.cos(angle), math.cos(p * f), abs_tol=1e-14) and math.isclose(math.sin(angle), math.sin(p * f), abs_tol=1e-14)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,positions", [
+    (torch.int64, [10 ** 12 + 7, 2 ** 40 + 1, 2 ** 50 + 3, -(2 ** 50) - 1, 2 ** 53 - 1, 2 ** 53 + 1, -(2 ** 53) - 1, 1733702400123456789, 2 ** 62 + 1, 2 ** 63 - 1,
+                   2 ** 63 - 2 ** 9, -(2 ** 63), -(2 ** 63) + 1, 2 ** 32, 2 ** 32 - 1, -(2 ** 32), -1, 0]),
+    (torch.int32, [2 ** 31 - 1, -(2 ** 31), 1234567891, -3, 0]), (torch.float32, [1.0e12, 2.0 ** 60 + 2.0 ** 37, -3.3e15, 0.1, -1e-30, 0.0])])
+@pytest.mark.parametrize("unit", [1.0, 100.0])
+def test_angles_of_positions_beyond_53_bits(dtype, positions, unit):
+    """The tolerance is the module's: the fraction of a turn is rounded to fp32, whatever the position."""
+    g = torch.Generator().manual_seed(4)
+    plan = axial_plan(64, axes=1, theta=10000.0, unit=unit)
+    where = torch.tensor(positions, dtype=dtype)[:, None]
+    q = torch.randn(1, len(positions), 3, 64, generator=g)
+    angle = 2 * math.pi * fractions_of_a_turn(where[:, 0].tolist(), plan.freqs.tolist())
+    c, s = angle.cos()[None, :, None], angle.sin()[None, :, None]
+    a, b = q.double().chunk(2, -1)
+    for inverse in (False, True):
+        got = rotary(q.cuda(), None, where.cuda(), plan, inverse=inverse)[0].cpu().double()
+        turned = torch.cat((a * c - b * s, b * c + a * s) if not inverse else (a * c + b * s, b * c - a * s), -1)
+        room = (a.abs() + b.abs()).repeat(1, 1, 1, 2) * 2.0 ** -21 + turned.abs() * 2.0 ** -24
+        assert bool(((got - turned).abs() <= room).all()), float(((got - turned).abs() - room).max())
 
 
 @pytest.mark.gpu
