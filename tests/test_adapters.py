@@ -114,6 +114,78 @@ def test_many_requests_of_few_and_of_many_rows():
     check(adapter_linear(x, w, slots, vector(ids), vector(bounds), b=b, act="gelu"), x, w, slots, ids, bounds, b=b, act="gelu")
 
 
+def _bounds(counts, first=0):
+    at = [first]
+    for c in counts:
+        at.append(at[-1] + c)
+    return at
+
+
+CROWDS = {
+    "single rows": _bounds([1] * 300),                                                      # up to 128 requests in a tile of 128 rows, 256 in one of 256
+    "pairs and gaps": _bounds([2, 0, 1, 0, 3] * 40, first=5),
+    "empty ones between": _bounds([40] + [0] * 70 + [30] + [0] * 33 + [1] * 40 + [0] * 32 + [300]),  # whole rounds of 32 look-ups without a row
+    "growing": _bounds([i * i // 16 for i in range(48)]),
+    "forty rows each": _bounds([40] * 13)}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", ["r", "s64", "s128", "p256"])
+@pytest.mark.parametrize("crowd", CROWDS)
+@pytest.mark.parametrize("rank,act", [(8, "gelu"), (24, "swiglu"), (40, "res"), (64, None), (128, "swiglu")])
+def test_every_form_with_few_and_many_requests_in_a_tile(form, crowd, rank, act, monkeypatch):
+    """The form is forced, so that each one has all of these, whatever the rule that picks one."""
+    monkeypatch.setenv("FBB_ADAPTER_FORM", form)
+    g = torch.Generator("cuda").manual_seed(rank + len(crowd))
+    bounds, (K, N, L) = CROWDS[crowd], (200, 656, 7)
+    M, S = bounds[-1] + 3, len(bounds) - 1
+    x, w, slots, b = make(M, K, N, rank, L, g)
+    ids = [(s * 5 + 2) % (L + 2) - 1 for s in range(S)]  # -1 and L are no adapter
+    kw = {"b": b, "act": None if act == "res" else act}
+    if act == "res":
+        kw["res"], kw["gamma"] = torch.randn(M, N, generator=g, device="cuda").half(), torch.randn(N, generator=g, device="cuda").half()
+    need = _lib.load().fbb_adapter_linear_workspace_bytes(M, N, K, _lib.EPI_SWIGLU if act == "swiglu" else _lib.EPI_NONE, rank, S)
+    assert need == (M * N * 4 if form == "r" else M * rank * 2)  # what the rows form and the blocks form keep
+    out = adapter_linear(x, w, slots, vector(ids), vector(bounds), **kw)
+    check(out, x, w, slots, ids, bounds, **kw)
+    assert torch.equal(out, adapter_linear(x, w, slots, vector(ids), vector(bounds), **kw))
+    assert _lib.device_status() == (0, 0, 0, 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", ["r", "s64", "s128", "p256"])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_infinite_values_stay_in_their_rows_in_every_form(form, bad, monkeypatch):
+    monkeypatch.setenv("FBB_ADAPTER_FORM", form)
+    g = torch.Generator("cuda").manual_seed(6)
+    bounds = CROWDS["pairs and gaps"]
+    M, S, K, N = bounds[-1], len(bounds) - 1, 128, 320
+    x, w, slots, b = make(M, K, N, 16, 3, g)
+    ids = [s % 3 for s in range(S)]
+    clean = adapter_linear(x, w, slots, vector(ids), vector(bounds), b=b)
+    hit = torch.zeros(M, dtype=torch.bool, device="cuda")
+    for s in range(S):
+        hit[bounds[s]:bounds[s + 1]] = ids[s] == 1
+    for matrix in (slots.up, slots.down):
+        kept = matrix[1].clone()
+        matrix[1] = bad
+        out = adapter_linear(x, w, slots, vector(ids), vector(bounds), b=b)
+        assert torch.equal(out[~hit], clean[~hit]) and not bool(out[hit].isfinite().any())
+        matrix[1] = kept
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bounds,K,N,r", [(_bounds([40] * 64), 1024, 1024, 8), (_bounds([6145 * i * i // 85344 for i in range(64)]), 1024, 1024, 32),
+                                          (_bounds([1] * 2000), 384, 1536, 16)])
+def test_batches_of_many_requests_in_the_form_that_the_rule_picks(bounds, K, N, r):
+    g = torch.Generator("cuda").manual_seed(K + r)
+    S = len(bounds) - 1
+    x, w, slots, b = make(bounds[-1], K, N, r, 48, g)
+    ids = [-1 if s % 5 == 4 else s * 7 % 48 for s in range(S)]
+    check(adapter_linear(x, w, slots, vector(ids), vector(bounds), b=b), x, w, slots, ids, bounds, b=b)
+    assert _lib.device_status() == (0, 0, 0, 0)
+
+
 @pytest.mark.gpu
 def test_without_any_adapter_it_is_the_linear_layer():
     from fastbb_b200.gemm import linear
