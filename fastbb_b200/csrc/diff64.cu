@@ -36,7 +36,7 @@
 namespace fbb {
 
 constexpr int kDiffStages = 3;
-constexpr int kDiffPart = 16 * 128 + 16 * 2;  // floats of 16 rows of a part and map: the outputs, then {maximum, sum} of each row
+constexpr int kDiffPart = 16 * 128 + 16 * 2;  // floats of 16 rows of a part and map: the outputs, then {maximum, sum (-sum: of far rows)} of each row
 
 struct DiffSmem {
     static constexpr int kQOff = 0;                       // Q_1 | Q_2
@@ -180,6 +180,11 @@ __device__ __forceinline__ float4 ld_shared_f4(uint32_t addr) {
     asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
     return v;
 }
+
+// A row's exponents are s sl - m, m its running maximum times sl, rounded: the same m for all of them, so its rounding drops out with the sum.
+// From 2^22 on that rounding would be an exponent's worth and more. Rows of such scores are far: theirs are (s - r) sl, r the maximum itself,
+// whose difference is exact for the scores that matter.
+constexpr float kDiffFar = 4194304.f;
 
 constexpr int kDiffEarly = 2;  // key groups of eight exponentiated ahead of the vote on the running maximum (see kEarly in flash64.cu)
 
@@ -366,7 +371,7 @@ diff64_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
         const uint32_t tl = tmem_base + ((uint32_t)lane_base << 16);  // this warp's lanes
         const uint32_t tS = tl + t * 128, tO = tl + 256 + t * 128;
         const float sl = a.scale_log2;
-        const float lazy = kLazyMax / sl;
+        const float lazy = fminf(kLazyMax / sl, FLT_MAX);
         bool ok = true;
         uint32_t g = 0;
         int n = 0;
@@ -415,7 +420,10 @@ diff64_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
             float tA = 0.f, tB = 0.f;
             // (no lower: the maximum of keys that are all at minus infinity is subtracted from it)
             float mA = -FLT_MAX, mB = -FLT_MAX, lA = 0.f, lB = 0.f;
-            auto unit = [&](int i) -> bool {  // one half-block
+            bool far = false;  // this warp's rows are far, from the first half-block that has one on: mA and mB are the maxima themselves
+            // One half-block; false: a wait ran out, or (far is set, nothing else is changed) rows turned out far.
+            auto unit = [&](auto far_rows, int i) -> bool {
+                constexpr bool kFar = decltype(far_rows)::value;
                 const uint32_t half = g & 1u, tSh = tS + 64u * half;
                 if (!mbar_wait(s_full(t, half), (g >> 1) & 1u, s_abort, DEV_TIMEOUT_TMEM_FULL, 2 * t + half)) return false;
                 tc_fence_after();
@@ -427,18 +435,24 @@ diff64_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
                 if (64 * (i + 1) > here) mask_frag(sc, 64 * i + 2 * cq, here);  // (the last one may have keys beyond the entry's)
                 max_frag<8>(sc, mxA, mxB);
                 float2 accA = make_float2(0.f, 0.f), accB = make_float2(0.f, 0.f);
-                exp_frag<kDiffEarly>(sc, sl, mA, mB, accA, accB, pk);
-                if (i == 0 || __any_sync(0xffffffffu, mxA > tA || mxB > tB)) {
+                if constexpr (!kFar) exp_frag<kDiffEarly>(sc, sl, mA, mB, accA, accB, pk);
+                if (i == 0 || __any_sync(0xffffffffu, kFar ? mxA - mA > lazy || mxB - mB > lazy || tA != 0.f || tB != 0.f : mxA > tA || mxB > tB)) {
                     mxA = fmaxf(mxA, __shfl_xor_sync(0xffffffffu, mxA, 1));
                     mxB = fmaxf(mxB, __shfl_xor_sync(0xffffffffu, mxB, 1));
                     mxA = fmaxf(mxA, __shfl_xor_sync(0xffffffffu, mxA, 2));
                     mxB = fmaxf(mxB, __shfl_xor_sync(0xffffffffu, mxB, 2));
-                    const float nA = fmaxf(mA, mxA * sl), nB = fmaxf(mB, mxB * sl);
+                    if constexpr (!kFar) {
+                        if (__any_sync(0xffffffffu, fmaxf(fabsf(mxA), fabsf(mxB)) * sl >= kDiffFar)) {  // (infinities too)
+                            far = true;
+                            return false;
+                        }
+                    }
+                    const float nA = fmaxf(mA, kFar ? mxA : mxA * sl), nB = fmaxf(mB, kFar ? mxB : mxB * sl);
                     if (i > 0) {
                         // the unit before this one may still be adding to O_t
                         if (!mbar_wait(pv_done(t, half ^ 1u), ((g - 1u) >> 1) & 1u, s_abort, DEV_TIMEOUT_TMEM_FULL, 8 + 2 * t + half)) return false;
                         tc_fence_after();
-                        const float cA = ex2_approx(mA - nA), cB = ex2_approx(mB - nB);
+                        const float cA = ex2_approx(kFar ? (mA - nA) * sl + tA : mA - nA), cB = ex2_approx(kFar ? (mB - nB) * sl + tB : mB - nB);
 #pragma unroll 1
                         for (int c = 0; c < 8; ++c) {
                             uint32_t o[8];
@@ -458,12 +472,22 @@ diff64_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
                     }
                     mA = nA;
                     mB = nB;
-                    tA = i == 0 ? mxA + lazy : fmaxf(tA, mxA + lazy);
-                    tB = i == 0 ? mxB + lazy : fmaxf(tB, mxB + lazy);
-                    accA = accB = make_float2(0.f, 0.f);
-                    exp_frag<kDiffEarly>(sc, sl, mA, mB, accA, accB, pk);
+                    if constexpr (kFar) {
+                        tA = tB = 0.f;
+                    } else {
+                        tA = i == 0 ? mxA + lazy : fmaxf(tA, mxA + lazy);
+                        tB = i == 0 ? mxB + lazy : fmaxf(tB, mxB + lazy);
+                        accA = accB = make_float2(0.f, 0.f);
+                        exp_frag<kDiffEarly>(sc, sl, mA, mB, accA, accB, pk);
+                    }
                 }
-                exp_frag<8 - kDiffEarly>(sc + 4 * kDiffEarly, sl, mA, mB, accA, accB, pk + 2 * kDiffEarly);
+                if constexpr (kFar) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) sc[j] = __float_as_uint(__uint_as_float(sc[j]) - ((j & 2) ? mB : mA));
+                    exp_frag<8>(sc, sl, 0.f, 0.f, accA, accB, pk);
+                } else {
+                    exp_frag<8 - kDiffEarly>(sc + 4 * kDiffEarly, sl, mA, mB, accA, accB, pk + 2 * kDiffEarly);
+                }
                 tmem_st_16x128b_x8(tSh, pk);
                 tmem_wait_st();
                 tc_fence_before();
@@ -473,8 +497,22 @@ diff64_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
                 lB += accB.x + accB.y;
                 return true;
             };
+            int i = 0;
 #pragma unroll 1
-            for (int i = 0; i < halves && ok; ++i, ++g) ok = unit(i);
+            for (; i < halves; ++i, ++g)
+                if (!(ok = unit(std::false_type{}, i))) break;
+            if (far) {
+                // The maxima so far become scores again (a maximum of no score yet stays the lowest number). The exponent by which that
+                // changes them goes into what O and the sums are raised by right after.
+                ok = true;
+                const float rA = mA == -FLT_MAX ? mA : mA / sl, rB = mB == -FLT_MAX ? mB : mB / sl;
+                tA = mA == -FLT_MAX ? 0.f : fmaf(-rA, sl, mA);
+                tB = mB == -FLT_MAX ? 0.f : fmaf(-rB, sl, mB);
+                mA = rA;
+                mB = rB;
+#pragma unroll 1
+                for (; i < halves && ok; ++i, ++g) ok = unit(std::true_type{}, i);
+            }
             if (ok && halves > 0) ok = mbar_wait(pv_done(t, (g - 1u) & 1u), ((g - 1u) >> 1) & 1u, s_abort, DEV_TIMEOUT_TMEM_FULL, 12 + t);
             // a row's sum is spread over the four threads that share it
             lA += __shfl_xor_sync(0xffffffffu, lA, 1);
@@ -499,8 +537,8 @@ diff64_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
                         }
                     }
                     float2* stat = reinterpret_cast<float2*>(dst + 16 * 128);
-                    if (cq == 0) stat[lane >> 2] = make_float2(mA, lA);
-                    if (cq == 1) stat[(lane >> 2) + 8] = make_float2(mB, lB);
+                    if (cq == 0) stat[lane >> 2] = make_float2(mA, far ? -lA : lA);
+                    if (cq == 1) stat[(lane >> 2) + 8] = make_float2(mB, far ? -lB : lB);
                     release();
                 }
                 continue;
@@ -624,14 +662,37 @@ __global__ void __launch_bounds__(512) diff64_join_kernel(const DiffArgs a) {
     if (used) load(0);
     float lam = 1.f;
     if (t == 1 && used) lam = a.lam[b * a.l_sb + (row0 + r) * a.l_sn + h * a.l_sh];
+    int far = 0;  // some of these rows are, in some share
     for (int i = threadIdx.x; i < live * 32; i += 512) {
         const int j = i >> 5, mr = i & 31;
-        s_stat[j][mr >> 4][mr & 15] = __ldcg(reinterpret_cast<const float2*>(part + (int64_t)share(j) * step + (mr >> 4) * (step / 2) + 16 * 128) + (mr & 15));
+        const float2 stat = __ldcg(reinterpret_cast<const float2*>(part + (int64_t)share(j) * step + (mr >> 4) * (step / 2) + 16 * 128) + (mr & 15));
+        s_stat[j][mr >> 4][mr & 15] = stat;
+        far |= signbit(stat.y);
     }
-    __syncthreads();
+    far = __syncthreads_or(far);
     if (used) {  // (whole rows of 16 threads, whose shuffles stay among themselves)
         const unsigned mask = 0xffffu << (threadIdx.x & 16);
         float m = -INFINITY, l = 0.f;
+        if (far) {  // maxima become exponents relative to the greatest, a far share's or another's
+            float top = -INFINITY, near = -FLT_MAX;
+            for (int j = strand; j < live; j += 16) {
+                const float2 stat = s_stat[j][t][r];
+                if (signbit(stat.y)) top = fmaxf(top, stat.x);
+                else near = fmaxf(near, stat.x);
+            }
+#pragma unroll
+            for (int d = 1; d < 16; d <<= 1) {
+                top = fmaxf(top, __shfl_xor_sync(mask, top, d));
+                near = fmaxf(near, __shfl_xor_sync(mask, near, d));
+            }
+            const bool from_top = fmaf(top, a.scale_log2, -near) > 0.f;
+            for (int j = strand; j < live; j += 16) {
+                const float2 stat = s_stat[j][t][r];
+                const float x = signbit(stat.y) ? (from_top ? (stat.x - top) * a.scale_log2 : fmaf(stat.x, a.scale_log2, -near))
+                                                : (from_top ? fmaf(-top, a.scale_log2, stat.x) : stat.x - near);
+                s_stat[j][t][r] = make_float2(x, fabsf(stat.y));
+            }
+        }
         for (int j = strand; j < live; j += 16) m = fmaxf(m, s_stat[j][t][r].x);
 #pragma unroll
         for (int d = 1; d < 16; d <<= 1) m = fmaxf(m, __shfl_xor_sync(mask, m, d));

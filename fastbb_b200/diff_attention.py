@@ -29,8 +29,7 @@ def diff_attention(q, k, v, lam, weight=None, eps=1e-5, out_scale=1.0, scale=Non
     dim contiguous, other strides multiples of 8 elements, no expanded dims). Hk divides H: query heads in a row share a key head.
     lam: fp32 tensor that broadcasts to [B, Nq, H] (a scalar, one per head, one per token and head).
     weight: [128] fp16 or fp32: each row of 128 is divided by its root mean square, sqrt(mean(o^2) + eps), and multiplied by it.
-    out_scale: a factor of the result, with or without the norm. scale: of the scores, 64^-0.5 unless given, > 0
-    (scaled scores may reach 6e7 in magnitude).
+    out_scale: a factor of the result, with or without the norm. scale: of the scores, 64^-0.5 unless given, > 0.
     key_lengths: int32 [B] on the GPU: keys from key_lengths[b] on are not seen, whatever they hold; a row without keys is 0.
     out: fp16 [B, Nq, H, 128] that shares no memory with any input."""
     uq, uk, uv = _usable(q, 64), _usable(k, 64), _usable(v, 128)

@@ -232,7 +232,7 @@ int fbb_adapter_linear_f16_from(const fbb_adapter_linear_args* args);
  * weight: [128] of weight_dtype (fp16 or fp32) or null. lengths: int32 [B] or null; keys from lengths[b] on are not seen, whatever k and
  * v hold there (a number below 0 counts as 0, beyond Nk as Nk); without any key a row of o is 0. scale > 0.
  * Scores, maxima, sums and outputs are fp32; the probabilities are rounded to fp16 for the second product, relative to a maximum that
- * is at most 2^8 too small. Scaled scores may reach 6e7 in magnitude; beyond that fp32 no longer tells the exponents apart.
+ * is at most 2^8 too small. Scaled scores of any magnitude.
  * workspace: fbb_diff64_workspace_bytes() of 16-byte aligned device memory (0 bytes where the keys are not split), overwritten
  * freely; calls that may overlap in time need different ones. fbb_diff64_launches: kernels a call enqueues (1, or 2 with split keys). */
 int64_t fbb_diff64_workspace_bytes(int B, int Nq, int Nk, int H);

@@ -269,6 +269,52 @@ def test_scores_of_minus_infinity_ahead_of_the_others(Nq, Nk, dead):
     assert _lib.device_status() == (0, 0, 0, 0)
 
 
+FAR = {  # (first column of a key, second column): with queries of 2^15 and 2^7 there, scores of 2^15 times the first and 2^7 times the second
+    "rising": lambda j, n: (torch.floor(16.0 * j / n) * 4000 - 2000, j % 5),
+    "falling": lambda j, n: (60000 - torch.floor(16.0 * j / n) * 4000, j % 7),
+    "ties": lambda j, n: (60000 + 0 * j, 0 * j),
+    "near ties": lambda j, n: (48000 + 0 * j, j % 3),
+    "far below nought": lambda j, n: (-60000 + 32 * (j % 11), 0 * j),
+    "from far below to near": lambda j, n: (torch.where(j < 0.7 * n, -50000.0, 0.0), j % 4),
+    "near, then far, then further": lambda j, n: (torch.where(j < 0.3 * n, 0.0, torch.where(j < 0.6 * n, 3000.0, 40000.0)), j % 2),
+    "around 2^22": lambda j, n: (700 + torch.floor(8.0 * j / n), j % 6),
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Nq,Nk,scale", [(150, 300, None), (1, 3000, None), (20, 129, 1.0), (5, 2500, 3e-5), (3, 500, 1e27)])
+@pytest.mark.parametrize("kind", FAR)
+def test_scores_of_any_magnitude(Nq, Nk, scale, kind):
+    """Scores that fp32 holds exactly, so that they have no tolerance, up to 3e8 times scale and far apart. Tolerance: exponents are differences of
+    exact scores times scale, off by 2^-22 of themselves; those of weights that count are below 32: 2^-17. The rest as above."""
+    g = torch.Generator("cuda").manual_seed(Nk)
+    j = torch.arange(Nk, device="cuda", dtype=torch.float64)
+    first, second = FAR[kind](j, Nk)
+    q, k = torch.zeros(1, Nq, 4, 64, device="cuda").half(), torch.zeros(1, Nk, 4, 64, device="cuda").half()
+    q[..., 3], q[..., 40] = 2.0 ** 15, 2.0 ** 7
+    q[:, ::2, 1] = 0  # some rows of all scores alike, beside the far ones
+    for head in range(4):
+        turn = head * (Nk // 5)  # each map meets its maxima elsewhere
+        k[0, :, head, 3], k[0, :, head, 40] = first.roll(turn).half(), second.roll(turn).half()
+    v, lam = torch.randn(1, Nk, 2, 128, generator=g, device="cuda").half(), torch.tensor([0.3, 0.6], device="cuda")
+    s_ = 0.125 if scale is None else float(torch.tensor(scale))
+    want, room = torch.zeros(1, Nq, 2, 128, dtype=torch.float64, device="cuda"), 0
+    for t in range(2):
+        s = torch.einsum("qhc,khc->hqk", q[0, :, t::2].double(), k[0, :, t::2].double())
+        assert torch.equal(s.float().double(), s)
+        p = torch.exp((s - s.amax(-1, keepdim=True)) * s_)
+        l = p.sum(-1, keepdim=True)
+        vv = v[0].double().transpose(0, 1)
+        x, f = (p @ vv / l).transpose(0, 1), 1.0 if t == 0 else lam.double()[:, None]
+        d = ((2.0 ** -11 + 2.0 ** -16 + 2.0 ** -21) * (p @ vv.abs() / l) + 2.0 ** -25 * vv.abs().sum(1, keepdim=True) / l).transpose(0, 1) + 2.0 ** -22 * x.abs()
+        want[0] += x if t == 0 else -f * x
+        room = room + f * d
+    out = diff_attention(q, k, v, lam, scale=scale)
+    over = (out[0].double() - want[0]).abs() - room - want[0].abs() * 2.0 ** -11 - 2.0 ** -25
+    assert bool((over <= 0).all()), f"{int((~(over <= 0)).sum())} of {over.numel()} off, worst by {float(over.max()):.3g}"
+    assert _lib.device_status() == (0, 0, 0, 0)
+
+
 @pytest.mark.gpu
 def test_refusals_on_the_gpu():
     g = torch.Generator("cuda").manual_seed(7)
