@@ -43,7 +43,7 @@ class Adapters:
 def adapter_linear(x, w, adapters, ids, offsets=None, b=None, act=None, res=None, gamma=None, out=None):
     """act(x w^T + b + scale_a (x down_a^T) up_a^T), a the adapter of the row's request; with res: res + gamma * that. As linear(): fp16 x [..., K],
     w [N, K], b and gamma vectors, res of the output's shape, act None | "gelu" | "swiglu"; fp32 accumulator. Each scale_a (x down_a^T) is rounded to
-    fp16 on the way (but for few rows of many requests): beyond fp16's range it is infinite.
+    fp16 on the way (but for few rows of many requests); a row of it with values beyond fp16's range is held times 2^-15, so up to 2^31.
 
     ids: int32 [S] on the GPU, the adapter of each request; a number out of [0, L) (say -1): none.
     offsets: int32 [S + 1] on the GPU, not decreasing: request s has rows offsets[s] .. offsets[s + 1] - 1 of x's rows taken in order; rows of

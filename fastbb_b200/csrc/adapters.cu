@@ -6,7 +6,11 @@
 // under the first (its product with W needs nothing of it) and waits for it where it needs h. Two forms of the pair:
 //  blocks  h is [M, r], and the linear kernel runs it as k-blocks behind those of x and W: of every request in a row tile one k-block of 64
 //          (for ranks up to 64) against its adapter's second matrix, which adds to the request's rows of the accumulator alone (the
-//          lanes of tensor memory that a product leaves as they are are an operand of the instruction)
+//          lanes of tensor memory that a product leaves as they are are an operand of the instruction). A row of h with values beyond fp16
+//          is held times 2^-15 and marked: the row's first product multiplies what it has so far by that too (an operand of the
+//          instruction as well), and the epilogue takes the whole sum back. So whether a request's output is finite does not
+//          depend on the form, or on what else is in the batch. (The marks cost 0.3 us of 16 at 8 x 257, 768 -> 2304, rank 16, 0.8 of 53 at
+//          6146 rows, 1024 -> 4096, rank 32, and 0.9 of 170 at 21920 rows, 4096 -> 1024, rank 64.)
 //  rows    for few rows of many requests, where that would be a k-block per row or so: the first launch multiplies each row with both
 //          of its adapter's matrices on the CUDA cores (bound by reading those), and the linear kernel's epilogue adds that in fp32.
 // Rows of no request (ahead of offsets[0], behind offsets[S]) and of requests with an id out of [0, adapters) get x W^T alone.
@@ -22,6 +26,7 @@ struct AdapterArgs {
     // blocks form
     int pass_cols, stages;  // columns of h in a pass, a multiple of 16 up to kDownCols; tiles of x on their way
     __half* h;
+    uint32_t* lifted;       // [M / 32, up to whole 256 rows]: a bit per row whose h is held times 2^-15
     // rows form
     const __half* x;
     int64_t ldx;
@@ -170,6 +175,7 @@ __global__ void __launch_bounds__(kDownThreads) adapter_down_kernel(const __grid
         }
     } else {
         const int quad = warp & 3, row = m0 + quad * 32 + lane;
+        uint32_t lifted = 0;
         for (int p = 0; p < passes; ++p) {
             const int req0 = p * per_pass, n = min(per_pass, requests - req0), acc = p & 1;
             const float scales = __ldcg(a.scale + s_req[req0 + min(lane, n - 1)].z);  // lane i: of request req0 + i (per_pass is 16 at most)
@@ -180,18 +186,38 @@ __global__ void __launch_bounds__(kDownThreads) adapter_down_kernel(const __grid
                 const float scale = __shfl_sync(0xffffffffu, scales, i);
                 const bool mine = row >= req.x && row < req.y;
                 uint4* dst = reinterpret_cast<uint4*>(a.h + (int64_t)row * a.r);
-                for (int c = 0; c < a.r; c += 8) {
-                    uint32_t v[8];
-                    tmem_ld8(tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * kDownCols + i * a.r + c), v);
-                    tmem_wait_ld();
-                    if (mine)
-                        dst[c >> 3] = make_uint4(pack_h2(__uint_as_float(v[0]) * scale, __uint_as_float(v[1]) * scale), pack_h2(__uint_as_float(v[2]) * scale, __uint_as_float(v[3]) * scale),
-                                                 pack_h2(__uint_as_float(v[4]) * scale, __uint_as_float(v[5]) * scale), pack_h2(__uint_as_float(v[6]) * scale, __uint_as_float(v[7]) * scale));
+                const uint32_t src = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * kDownCols + i * a.r);
+                // once, and a second time for rows with a value beyond fp16, times 2^-15
+                bool on = mine;
+                float f = scale;
+#pragma unroll 1
+                for (int once = 0; once < 2; ++once) {
+                    __half2 most = __float2half2_rn(0.f);
+                    for (int c = 0; c < a.r; c += 8) {
+                        uint32_t v[8];
+                        tmem_ld8(src + (uint32_t)c, v);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            v[j] = pack_h2(__uint_as_float(v[2 * j]) * f, __uint_as_float(v[2 * j + 1]) * f);
+                            most = __hmax2(most, __habs2(*reinterpret_cast<const __half2*>(&v[j])));
+                        }
+                        if (on) dst[c >> 3] = make_uint4(v[0], v[1], v[2], v[3]);
+                    }
+                    on = on && __hisinf(__hmax(__low2half(most), __high2half(most)));
+                    const uint32_t beyond = __ballot_sync(0xffffffffu, on);
+                    if (beyond == 0u || once == 1) break;
+                    lifted |= beyond;
+                    f = scale * 0x1p-15f;
                 }
             }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(tempty_bar(acc));
+        }
+        if (lane == 0) {
+            a.lifted[(m0 >> 5) + quad] = lifted;
+            if (blockIdx.x + 1 == gridDim.x && (blockIdx.x & 1u) == 0u) a.lifted[(m0 >> 5) + 4 + quad] = 0;
         }
     }
     tc_fence_before();
@@ -294,8 +320,8 @@ static AdapterForm adapter_form(int64_t M, int N, int K, bool swiglu, int r, int
     return f;
 }
 
-// Workspace: h, or the rows form's delta.
-static int64_t adapter_space(const AdapterForm& f, int64_t M, int N, int r) { return f.rows ? M * N * (int64_t)sizeof(float) : M * r * 2; }
+// Workspace: h and the bits of lifted rows, or the rows form's delta.
+static int64_t adapter_space(const AdapterForm& f, int64_t M, int N, int r) { return f.rows ? M * N * (int64_t)sizeof(float) : M * r * 2 + (M + 255) / 256 * 32; }
 
 int64_t adapter_linear_workspace_bytes(int64_t M, int N, int K, int epilogue, int r, int S) {
     if (M <= 0 || S <= 0) return 0;
@@ -344,6 +370,7 @@ int launch_adapter_linear(const void* A, const void* W, void* C, const void* bia
     d.scale = scale;
     d.M = (int)M, d.N = N, d.K = K, d.r = r;
     d.h = reinterpret_cast<__half*>(ws);
+    d.lifted = reinterpret_cast<uint32_t*>(d.h + M * r);  // (r is a multiple of 8)
     d.x = reinterpret_cast<const __half*>(A);
     d.ldx = lda;
     d.down = reinterpret_cast<const __half*>(down);
@@ -409,6 +436,7 @@ int launch_adapter_linear(const void* A, const void* W, void* C, const void* bia
     AdaptArgs ad = {};
     ad.requests = d.requests;
     ad.delta = d.delta;
+    ad.lifted = d.lifted;
     ad.r_blocks = (r + BK - 1) / BK;
 
 #define FBB_ADAPTER_LAUNCH(BN, SWIGLU, CTA2, MODE) launch_adapter_variant<BN, SWIGLU, CTA2, MODE>(ta, tw, th, tu, tc, g, ad, stream)

@@ -245,6 +245,11 @@ __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t* r) {
         : "r"(taddr)
         : "memory");
 }
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+        : "memory");
+}
 // 16-lane shapes: the warp touches 16 tensor-memory lanes starting at the lane in the address. Register layout (checked on
 // hardware): 16x256b.xN -> thread t holds r[4k+j]: lane t/4 + 8*(j/2), column 8k + 2*(t%4) + j%2 (the mma m16n8 accumulator
 // fragment); 16x128b.xN -> r[2k+j]: lane t/4 + 8*j, column 4k + t%4.
@@ -368,6 +373,27 @@ __device__ __forceinline__ void umma_kblock_rows_commit_warp(uint32_t d_tmem, ui
         "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%8];\n\t"
         "}\n"
         ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3]), "r"(bar)
+        : "memory");
+}
+// The same without the commit, onto the accumulator's rows times 2^-15.
+__device__ __forceinline__ void umma_kblock_rows_lift_warp(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, const uint32_t* off) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred q;\n\t"
+        ".reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
+        "add.s64 a1, %1, 2;\n\t"
+        "add.s64 b1, %2, 2;\n\t"
+        "add.s64 a2, %1, 4;\n\t"
+        "add.s64 b2, %2, 4;\n\t"
+        "add.s64 a3, %1, 6;\n\t"
+        "add.s64 b3, %2, 6;\n\t"
+        "elect.sync _|q, 0xFFFFFFFF;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %7}, 1, 15;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, {%4, %5, %6, %7}, 1;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, {%4, %5, %6, %7}, 1;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, {%4, %5, %6, %7}, 1;\n\t"
+        "}\n"
+        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3])
         : "memory");
 }
 // The same with commits to two barriers, accumulator overwritten (the Q K^T of one key block).
@@ -539,6 +565,27 @@ __device__ __forceinline__ void umma_kblock_rows_commit_pair_warp(uint32_t d_tme
         "}\n"
         ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3]), "r"(off[4]), "r"(off[5]), "r"(off[6]), "r"(off[7]), "r"(bar),
           "r"(mask)
+        : "memory");
+}
+// The same without the commit, onto the accumulator's rows times 2^-15.
+__device__ __forceinline__ void umma_kblock_rows_lift_pair_warp(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, const uint32_t* off) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred q;\n\t"
+        ".reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
+        "add.s64 a1, %1, 2;\n\t"
+        "add.s64 b1, %2, 2;\n\t"
+        "add.s64 a2, %1, 4;\n\t"
+        "add.s64 b2, %2, 4;\n\t"
+        "add.s64 a3, %1, 6;\n\t"
+        "add.s64 b3, %2, 6;\n\t"
+        "elect.sync _|q, 0xFFFFFFFF;\n\t"
+        "@q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %7, %8, %9, %10, %11}, 1, 15;\n\t"
+        "@q tcgen05.mma.cta_group::2.kind::f16 [%0], a1, b1, %3, {%4, %5, %6, %7, %8, %9, %10, %11}, 1;\n\t"
+        "@q tcgen05.mma.cta_group::2.kind::f16 [%0], a2, b2, %3, {%4, %5, %6, %7, %8, %9, %10, %11}, 1;\n\t"
+        "@q tcgen05.mma.cta_group::2.kind::f16 [%0], a3, b3, %3, {%4, %5, %6, %7, %8, %9, %10, %11}, 1;\n\t"
+        "}\n"
+        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3]), "r"(off[4]), "r"(off[5]), "r"(off[6]), "r"(off[7])
         : "memory");
 }
 // The four K16 steps alone.

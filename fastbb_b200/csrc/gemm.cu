@@ -163,6 +163,7 @@ struct AdaptArgs {
     const CUtensorMap* map_h;  // h [M, r]
     const CUtensorMap* map_up; // the adapters' second matrices [adapters * N, r]
     int r_blocks;              // 64-element k-blocks of the rank
+    const uint32_t* lifted;    // a bit per row: its h is held times 2^-15
     // rows
     const float* delta;        // [M, N]: added to the accumulator
 };
@@ -362,7 +363,15 @@ __device__ __forceinline__ void linear_umma_body(const CUtensorMap& tmap_a, cons
         int acc = 0;
         uint32_t acc_ph = 0;
         bool ok = true;
+        // (adapters) lane i: which of the tile's rows 32 i .. 32 i + 31 are lifted; readable once the kernel that makes h is done
+        uint32_t lifted = 0;
+        bool h_done = false;
         for (int item = worker; item < num_items && ok; item += num_workers) {
+            auto load_lifted = [&]() {
+                if (lane < kTileRows / 32) lifted = __ldcg(ad.lifted + item / g.tiles_n * (kTileRows / 32) + lane);
+            };
+            if constexpr (ADAPT == kAdaptBlocks)
+                if (h_done) load_lifted();  // under the tile's plain k-blocks
             const uint32_t idesc = (kNarrowOk && item >= g.wide_tiles) ? idesc_slice : idesc_tile;
             if (!all_ok(mbar_wait(tempty_bar(acc), acc_ph ^ 1u, s_abort, DEV_TIMEOUT_TMEM_EMPTY, acc))) break;
             tc_fence_after();
@@ -389,9 +398,16 @@ __device__ __forceinline__ void linear_umma_body(const CUtensorMap& tmap_a, cons
                 if (!ok) break;
                 const int extra = s_extra[s];
                 ok = multiply(plain_kb);
+                if (extra > 0 && !h_done) {
+                    grid_dependency_wait();
+                    h_done = true;
+                    load_lifted();
+                }
+                bool lifts = false;
                 for (int kb = 0; kb < extra && ok; ++kb) {
                     ok = all_ok(mbar_wait(full_bar(s), ph, s_abort, DEV_TIMEOUT_TMA_FULL, s));
                     if (!ok) break;
+                    if (kb == 0) lifts = __any_sync(0xffffffffu, lifted != 0u);  // (its load has run under the wait for h)
                     tc_fence_after();
                     // Into the request's rows alone: others' rows hold others' h, and an infinity in one adapter is none of theirs.
                     const int b = s_rows[2 * s], e = s_rows[2 * s + 1];
@@ -402,6 +418,18 @@ __device__ __forceinline__ void linear_umma_body(const CUtensorMap& tmap_a, cons
                         off[i] = ~(uint32_t)((1ull << hi) - (1ull << min(lo, hi)));
                     }
                     const uint64_t adesc = adesc0 + (uint64_t)(s * (S::kStageBytes >> 4)), bdesc = adesc + (uint64_t)(S::kABytes >> 4);
+                    if (lifts && kb % ad.r_blocks == 0) {
+                        // rows whose h is held times 2^-15 go on so, what they have so far as well; the epilogue takes them back
+                        uint32_t others[CTA2 ? 8 : 4];
+#pragma unroll
+                        for (int i = 0; i < (CTA2 ? 8 : 4); ++i) {
+                            const uint32_t word = __shfl_sync(0xffffffffu, lifted, i);
+                            others[i] = off[i] | ~word;
+                            off[i] |= word;
+                        }
+                        if constexpr (CTA2) umma_kblock_rows_lift_pair_warp(d_tmem, adesc, bdesc, idesc, others);
+                        else umma_kblock_rows_lift_warp(d_tmem, adesc, bdesc, idesc, others);
+                    }
                     if constexpr (CTA2) umma_kblock_rows_commit_pair_warp(d_tmem, adesc, bdesc, idesc, off, empty_bar(s), 3u);
                     else umma_kblock_rows_commit_warp(d_tmem, adesc, bdesc, idesc, off, empty_bar(s));
                     if (++s == kStages) { s = 0; ph ^= 1u; }
@@ -423,11 +451,15 @@ __device__ __forceinline__ void linear_umma_body(const CUtensorMap& tmap_a, cons
         if (g.gemv_rows > 0) remainder_rows_by_gemv(g, SWIGLU, (int)blockIdx.x * 8 + ew, (int)gridDim.x * 8, lane);
         int acc = 0;
         uint32_t acc_ph = 0;
+        bool h_done = false;
         for (int item = worker; item < num_items; item += num_workers) {
             int m0, n0, w;  // n0: first output column of the item
             item_at(item, m0, n0, w);
             const int half_cols = SWIGLU ? kOutCols / 2 : w / 2;  // output columns per half of the epilogue warps
             const int chunks = half_cols / 32;
+            uint32_t lifted = 0;  // (adapters) this warp's rows that are held times 2^-15
+            if constexpr (ADAPT == kAdaptBlocks)
+                if (h_done) lifted = __ldcg(ad.lifted + (m0 >> 5) + quad);
             // stage bias (W-row indexed) and gamma (output-column indexed) for this item
             float* s_bias = s_params + acc * 2 * BN;
             float* s_gamma = s_bias + BN;
@@ -471,9 +503,32 @@ __device__ __forceinline__ void linear_umma_body(const CUtensorMap& tmap_a, cons
                 }
             };
             if constexpr (ADAPT == kAdaptRows) grid_dependency_wait();
+            if constexpr (ADAPT == kAdaptBlocks) {
+                if (!h_done) {
+                    grid_dependency_wait();
+                    h_done = true;
+                    lifted = __ldcg(ad.lifted + (m0 >> 5) + quad);
+                }
+            }
             if (!mbar_wait(tfull_bar(acc), acc_ph, s_abort, DEV_TIMEOUT_TMEM_FULL, acc)) break;
             tc_fence_after();
             const uint32_t t_row = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * BN);
+            if constexpr (ADAPT == kAdaptBlocks) {
+                if (lifted != 0u) {  // taken back in place, this warp's columns
+                    const float lift = lifted >> lane & 1u ? 32768.f : 1.f;
+#pragma unroll 1
+                    for (int c = 0; c < (SWIGLU ? 2 : 1) * half_cols; c += 8) {
+                        const uint32_t at = t_row + (uint32_t)(chalf * half_cols + (c < half_cols ? c : BN / 2 - half_cols + c));
+                        uint32_t r[8];
+                        tmem_ld8(at, r);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * lift);
+                        tmem_st8(at, r);
+                    }
+                    tmem_wait_st();
+                }
+            }
 #pragma unroll
             for (int ci = 0; ci < kChunks; ++ci) {
                 if (ci >= chunks) break;

@@ -201,8 +201,8 @@ int fbb_flash64_f16_static(const void* q, const void* k, const void* v, void* o,
  * offsets: int32 [requests + 1], not decreasing: request s has rows offsets[s] .. offsets[s + 1] - 1; rows of no request have no adapter. null:
  * M / requests rows each (a whole number). Both are read on the device; offsets that decrease give wrong results for the rows they
  * concern, nothing else. adapters * N and adapters * rank < 2^31.
- * A . down_a^T times scale is rounded to fp16 ahead of the second product, infinite beyond fp16's range (not for few rows of many requests,
- * which are multiplied out on the CUDA cores); everything else is fp32. A NaN or infinity in a request's rows or its adapter stays in its rows.
+ * A . down_a^T times scale is rounded to fp16 ahead of the second product, a row with values beyond fp16's range times 2^-15, so up to 2^31
+ * (few rows of many requests are multiplied out on the CUDA cores instead); everything else is fp32. A NaN or infinity in a request's rows or its adapter stays in its rows.
  * workspace: fbb_adapter_linear_workspace_bytes() of 256-byte aligned device memory, overwritten freely; calls that may overlap in time need
  * different ones. Two kernels are enqueued. */
 int64_t fbb_adapter_linear_workspace_bytes(int64_t M, int N, int K, int epilogue, int rank, int requests);

@@ -145,7 +145,7 @@ def test_every_form_with_few_and_many_requests_in_a_tile(form, crowd, rank, act,
     if act == "res":
         kw["res"], kw["gamma"] = torch.randn(M, N, generator=g, device="cuda").half(), torch.randn(N, generator=g, device="cuda").half()
     need = _lib.load().fbb_adapter_linear_workspace_bytes(M, N, K, _lib.EPI_SWIGLU if act == "swiglu" else _lib.EPI_NONE, rank, S)
-    assert need == (M * N * 4 if form == "r" else M * rank * 2)  # what the rows form and the blocks form keep
+    assert need == (M * N * 4 if form == "r" else M * rank * 2 + (M + 255) // 256 * 32)  # what the rows form and the blocks form keep
     out = adapter_linear(x, w, slots, vector(ids), vector(bounds), **kw)
     check(out, x, w, slots, ids, bounds, **kw)
     assert torch.equal(out, adapter_linear(x, w, slots, vector(ids), vector(bounds), **kw))
@@ -172,6 +172,43 @@ def test_infinite_values_stay_in_their_rows_in_every_form(form, bad, monkeypatch
         out = adapter_linear(x, w, slots, vector(ids), vector(bounds), b=b)
         assert torch.equal(out[~hit], clean[~hit]) and not bool(out[hit].isfinite().any())
         matrix[1] = kept
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", ["r", "s64", "s128", "p256"])
+@pytest.mark.parametrize("crowd", CROWDS)
+@pytest.mark.parametrize("rank,act", [(8, "gelu"), (40, "res"), (72, None), (128, "swiglu")])
+def test_first_products_beyond_fp16(form, crowd, rank, act, monkeypatch):
+    """Rows of h up to about 3e7 beside rows that fp16 holds, in one request and in others of the tile. Rows beyond fp16 are held times 2^-15: fp16's
+    smallest step is 2^-10 of theirs, half of that on top of the tolerance (2^-25 of it is there already)."""
+    monkeypatch.setenv("FBB_ADAPTER_FORM", form)
+    g = torch.Generator("cuda").manual_seed(rank + len(crowd))
+    bounds, (K, N, L) = CROWDS[crowd], (200, 656, 3)
+    M, S = bounds[-1], len(bounds) - 1
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    x = (rnd(M, K) * torch.tensor([1.0, 10.0, 1000.0, 10000.0], device="cuda")[torch.randint(0, 4, (M, 1), generator=g, device="cuda")]).clamp(-60000, 60000).half()
+    scales = [0.7, 100.0, 3.0] if act != "swiglu" else [0.7, 10.0, 3.0]
+    slots = Adapters(rnd(L, rank, K).half(), (rnd(L, N, rank) * (2e-5 if act != "swiglu" else 2e-6)).half(), torch.tensor(scales, device="cuda"))
+    w, b, ids = (rnd(N, K) * 1e-4).half(), rnd(N).half(), [s % 4 for s in range(S)]  # 3 is no adapter
+    kw = {"b": b, "act": None if act == "res" else act}
+    if act == "res":
+        kw["res"], kw["gamma"] = rnd(M, N).half(), rnd(N).half()
+    want, room = reference(x, w, slots, ids, bounds, **kw)
+    most = max(float((slots.scale[a] * (x[bounds[s]:bounds[s + 1]].float() @ slots.down[a].float().t())).abs().max()) for s, a in enumerate(ids)
+               if a < L and bounds[s] < bounds[s + 1])
+    assert most > 1e6 and float(want.abs().max()) < 6e4
+    small = 2.0 ** -11 * float(slots.up.float().abs().sum(-1).max())
+    if act == "swiglu":
+        y = x.double() @ w.double().t() + b.double()
+        small *= 1.2 * float(want.abs().max() ** 0.5 + y.abs().max() + 60)  # (times the other half's values)
+    elif act == "res":
+        small = small * kw["gamma"].double().abs()
+    else:
+        small *= 1.13
+    out = adapter_linear(x, w, slots, vector(ids), vector(bounds), **kw)
+    over = (out.double() - want).abs() - room - small
+    assert bool((over <= 0).all()), f"{int((~(over <= 0)).sum())} of {over.numel()} off, worst by {float(over.max()):.3g}"
+    assert _lib.device_status() == (0, 0, 0, 0)
 
 
 @pytest.mark.gpu
