@@ -10,6 +10,8 @@ import torch
 
 from . import _lib
 
+_MOST = torch.finfo(torch.float32).max
+
 
 def _usable(t, columns):
     """(shape, stride, address) of a view that the kernel takes, None of any other."""
@@ -29,7 +31,7 @@ def diff_attention(q, k, v, lam, weight=None, eps=1e-5, out_scale=1.0, scale=Non
     dim contiguous, other strides multiples of 8 elements, no expanded dims). Hk divides H: query heads in a row share a key head.
     lam: fp32 tensor that broadcasts to [B, Nq, H] (a scalar, one per head, one per token and head).
     weight: [128] fp16 or fp32: each row of 128 is divided by its root mean square, sqrt(mean(o^2) + eps), and multiplied by it.
-    out_scale: a factor of the result, with or without the norm. scale: of the scores, 64^-0.5 unless given, > 0.
+    out_scale: a factor of the result, with or without the norm. scale: of the scores, 64^-0.5 unless given, > 0. All of them finite.
     key_lengths: int32 [B] on the GPU: keys from key_lengths[b] on are not seen, whatever they hold; a row without keys is 0.
     out: fp16 [B, Nq, H, 128] that shares no memory with any input."""
     uq, uk, uv = _usable(q, 64), _usable(k, 64), _usable(v, 128)
@@ -44,8 +46,8 @@ def diff_attention(q, k, v, lam, weight=None, eps=1e-5, out_scale=1.0, scale=Non
         raise ValueError("q must be [B, Nq, 2H, 64], k [B, Nk, 2Hk, 64] and v [B, Nk, Hk, 128] on one device, Hk a divisor of H")
     if scale is None:
         scale = 0.125
-    if not scale > 0 or not eps >= 0:
-        raise ValueError("scale must be > 0 and eps >= 0")
+    if not 0 < scale <= _MOST or not 0 <= eps <= _MOST or not abs(out_scale) <= _MOST:
+        raise ValueError("scale must be > 0, eps >= 0, and both and out_scale finite in fp32")
     if not torch.is_tensor(lam) or lam.dtype != torch.float32 or lam.device != device:
         raise ValueError("lam must be an fp32 tensor on the inputs' device")
     if lam.dim() == 1 and lam.shape[0] == H:

@@ -358,6 +358,17 @@ def test_outputs_over_any_input_are_refused():
         call(clear)
 
 
+@pytest.mark.gpu
+def test_factors_that_fp32_does_not_hold_are_refused():
+    g = torch.Generator("cuda").manual_seed(7)
+    q, k, v, lam = make(1, 4, 6, 2, 2, g)
+    for bad in ({"scale": 1e39}, {"scale": float("inf")}, {"eps": 1e39}, {"eps": float("nan")}, {"out_scale": -1e39}, {"out_scale": float("inf")}):
+        with pytest.raises(ValueError, match="finite"):
+            diff_attention(q, k, v, lam, **bad)
+    for good in ({"scale": 3e38}, {"eps": 3e38}, {"out_scale": -3e38}, {"out_scale": 0.0}):
+        diff_attention(q, k, v, lam, **good)
+
+
 # ------------------------------------------------------------------------------------------------------------------ CPU
 def test_cpu_tensors_are_refused():
     q = torch.zeros(1, 4, 2, 64).half()
