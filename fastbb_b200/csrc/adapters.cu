@@ -38,8 +38,10 @@ struct AdapterArgs {
 
 // h of the blocks form: a CTA takes 128 rows of x and multiplies them with the first matrices of their requests, up to 64 columns of
 // h at a time, or 128 where tiles hold many requests (several requests side by side where the rank leaves room), as UMMAs fed by TMA: x is
-// read once for most tiles. Many tiles are bound by that read (180 MB at 21920 x 4096: 28 us), few by latency: x's tiles start ahead of
-// the look-up of the requests, which is a chain of dependent loads, and as many are on their way as shared memory holds.
+// read once for most tiles. Many tiles: that read, 180 MB or 28 us at 21920 x 4096, rank 64, 16 requests, where the launch takes 50 under ncu:
+// the 15 of its 172 tiles that hold rows of two requests make two passes, the second one alone at the end. Few tiles are bound by
+// latency: x's tiles start ahead of the look-up of the requests, which is a chain of dependent loads, and as many are on their way as
+// shared memory holds (49 tiles of K = 1024: 12 - 13 us under ncu).
 //   warp 0   look-up of the requests, then TMA producer      warp 1   UMMA issuer      warps 2..5   rows of h out of tensor memory
 constexpr int kDownCols = 128;
 constexpr int kDownMaxStages = 12;
@@ -305,8 +307,9 @@ static AdapterForm adapter_form(int64_t M, int N, int K, bool swiglu, int r, int
     AdapterForm f = {};
     auto tiles = [&](int rows, int bn) { return ((M + rows - 1) / rows) * (int64_t)((n_out + (swiglu ? bn / 2 : bn) - 1) / (swiglu ? bn / 2 : bn)); };
     // What the forms add to the layer itself, us, fitted to measurements on B200 (rows / blocks, K = N = 1024, rank 16): 512 rows of 64
-    // requests 8.4 / 18, of 16 9 / 6.2; 2000 of 1000 19 / 58 (est.); 1200 of 75 (K = 768, N = 2304) 21.6 / 10.9. Rows: both matrices of every row's
-    // adapter are read once per row. Blocks: a product with either matrix per request and row tile.
+    // requests 8.2 / 19, of 32 8.2 / 10, of 16 8.0 / 6.7; 2000 of 1000 19 / 82; K = 768, N = 2304: 1200 of 150 22 / 21, of 75 22 / 11. Rows: both
+    // matrices of every row's adapter are read once per row. Blocks: a product with either matrix per request and row tile. Beyond 2^26
+    // outputs the rows form's workspace would pass 256 MB: blocks, also where single rows make them slow.
     const double rows_us = 4.3 + (double)M * r * ((double)K + N) * 2.0 / 6e6, per_tile = 1.0 + 128.0 * S / (double)M;
     f.rows = M * (int64_t)N <= (1 << 26) && rows_us < 3.2 + per_tile * (0.4 + 0.03 * r);
     const int pairs = gemm_pairs_enabled() ? (swiglu ? max_pairs<256, true>() : max_pairs<256, false>()) : 0;

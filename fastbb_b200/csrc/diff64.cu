@@ -3,9 +3,9 @@
 //
 // A tile is 128 queries of one (batch, head); it walks its keys in blocks of 128, both maps at once, so that v is read once and no map
 // or half of an output ever leaves the chip (as four calls of the flash64 kernel, one per map and half of v, every score is computed
-// twice and three passes over the outputs follow). One persistent CTA per SM takes every so-manieth tile. Where the tiles are fewer than
-// the SMs (few queries over many keys), each is split over the keys instead, and the splits' unnormalised rows, maxima and sums go
-// through the workspace to diff64_join_kernel.
+// twice and three passes over the outputs follow). One persistent CTA per SM takes every so-manieth tile. Where the SMs are twice the
+// tiles or more (few queries over many keys), each is split over the keys instead, and the splits' unnormalised rows, maxima and sums go
+// through the workspace to diff64_join_kernel. (From 75 to 147 tiles on 148 SMs there is one CTA a tile, and the other SMs rest.)
 //   warp 0          TMA producer: the two Q tiles, then K1, K2 and V of each block into a ring of stages (128-byte swizzle)
 //   warps 1, 2      UMMA issuers, one per map: S_t = Q_t K_t^T of half a block (64 keys) into one of two halves of the map's tensor memory;
 //                   once the softmax warps have put P_t (fp16) over it, O_t += P_t V (A from tensor memory, V as the MN-major B
@@ -25,9 +25,11 @@
 // Keys beyond a batch entry's number are masked by selection, never by adding, and their rows of V are zeroed in shared memory ahead
 // of the product, so that no infinity or NaN in them is seen.
 //
-// Bound by the exponentials where tiles are many: 6145 queries x 8 heads take 234 us, 993 TFLOP/s, with the transcendental unit busy for
-// 71 % of the clocks an SM is active and the tensor pipe for 54 %; few queries by the read of K and V (1 x 16385 x 8: 23 us, 10 of them
-// the read). Short tiles pay for their ends: 6.6 k clocks behind 2.8 k a block.
+// Bound by the exponentials where tiles are many: 6145 queries x 8 heads take 237 us in a row of launches (979 TFLOP/s; a launch's first tiles
+// run on SMs that the one ahead has left) and 272 by itself, with the transcendental unit busy for 70 % of the clocks an SM is active and
+// the tensor pipe for 53 %. Few queries are bound by the chain of half-blocks, of whose 16 softmax warps two have a row: 1 x 16385 x 8
+// takes 23.8 us, 14 half-blocks of 1.6 k clocks after one another 12 of them (the read of K and V, 10, runs beside), the merge about
+// 5, set-up and the tile's end the rest. Short tiles pay for their ends: 6.6 k clocks behind 2.8 k a block.
 #include <cfloat>
 
 #include "common.cuh"

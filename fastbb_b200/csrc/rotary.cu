@@ -4,13 +4,14 @@
 // sequence (cls and register tokens, which have no position) pass.
 //
 // Bound by memory: every element is read once and written once (50.4 MB at 6145 tokens x 16 + 16 heads x 64, fp16: 7.7 us at the
-// measured copy rate, 12.2 measured; fp32 at 4 x 1374 tokens x 48 x 64: 20.6 and 24.5). The angles of a token are the same for all its
+// measured copy rate, 12.1 measured: 769 CTAs on 444 places are two waves, the second three quarters full; fp32 at 4 x 1374 tokens x 48 x 64:
+// 20.6 and 24.4). The angles of a token are the same for all its
 // heads, so a CTA takes a few whole tokens, works their cos / sin out once into shared memory, and streams the tokens' heads through with
 // 16-byte accesses, kRotaryUnroll items in flight per thread (2 and 8 were slower: 54 - 66 and 53 us on 2 x 8184 x 20 x 128 bf16, now 37).
 // The angle, position times fp32 frequency, and its number of turns are doubles up to 2^20 radians, off by 2^-31 radians at most. Beyond, each is
 // a double and the remainder that its rounding left (Dekker's arithmetic: a product's remainder is one fma; 1 / (2 pi) is two doubles as
 // well), off by 2^-105 of the number of turns: fp32 angles lose nothing up to position times frequency of 2^70, which every int64 position
-// is within for frequencies up to 2^7. (All angles that way: 3 % more on the fp32 case below.) The turns' fraction is taken there;
+// is within for frequencies up to 2^7. (All angles that way: 3 % more on the fp32 case above.) The turns' fraction is taken there;
 // sincospif of twice that, at most 1, then has fp32 accuracy. The products and the sum are fp32, rounded once to the output type.
 #include <cuda_bf16.h>
 

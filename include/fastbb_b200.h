@@ -265,8 +265,9 @@ int fbb_diff64_f16_from(const fbb_diff64_args* args);
  * first n_prefix rows of every sequence pass unchanged. Angles are reduced to a turn in two doubles ahead of sine and cosine in fp32;
  * the rotation is fp32, rounded once.
  * tensors: one or two of {x, y, heads, strides of [B, N, heads, D] in elements, D contiguous}; y may be x itself, otherwise it
- * shares no memory with any x; positions, freqs and axes lie outside it, gaps of its strides included (refused otherwise). positions: [B, N - n_prefix, n_axes] of pos_dtype with strides p_sb, p_sn, p_sa (p_sb 0: the same
- * for every sequence). freqs: [pairs] fp32, axes: [pairs] int32, both in device memory; an axis out of [0, n_axes) is clamped.
+ * shares no memory with any x; positions, freqs and axes lie outside it, gaps of its strides included (refused otherwise).
+ * positions: [B, N - n_prefix, n_axes] of pos_dtype with strides p_sb, p_sn, p_sa (p_sb 0: the same for every sequence). freqs:
+ * [pairs] fp32, axes: [pairs] int32, both in device memory; an axis out of [0, n_axes) is clamped.
  * Any size, stride and alignment of whole elements; multiples of 16 bytes take the vector form. D <= 1024, B * N < 2^31. */
 enum fbb_rotary_pairing { FBB_ROTARY_HALF = 0, FBB_ROTARY_PAIRS = 1 };
 enum fbb_pos_dtype { FBB_POS_I32 = 0, FBB_POS_I64 = 1, FBB_POS_F32 = 2 };
